@@ -660,6 +660,94 @@ ML_API int ml_gemv_rmsnorm_swiglu_bf16(const void* x, int64_t ld_x, const void* 
                                        int64_t inter, void* y, int64_t ld_y, void* stream);
 
 /*
+ * A KV cache held in 8 bits, for decoding (no reference counterpart; the
+ * reference's static cache keeps the model's dtype, generation.py:18-66):
+ * codes [batch, kv_heads, max_len, head_dim] (int8, or e4m3 with
+ * ML_KV8_E4M3), one fp32 scale for each block of `block` positions and head
+ * ([batch, kv_heads, max_len / block]); value = code * scale.  k_tail / v_tail
+ * [batch, kv_heads, 2, block, head_dim] in `dtype` (ML_DTYPE_BF16 or
+ * ML_DTYPE_F16, the type of k, v, q and the output) keep the unquantised rows
+ * of the last two blocks written, block i in slot i & 1.  All contiguous;
+ * codes and tails 16-byte aligned; head_dim 64, 128 or 256; block 32, 64 or
+ * 128; max_len a multiple of block.
+ */
+#define ML_KV8_INT8 0
+#define ML_KV8_E4M3 1
+typedef struct ml_kv8_cache {
+  void* k_codes;
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  void* k_tail; /* only the append uses the tails */
+  void* v_tail;
+  int format;
+  int dtype;
+  int64_t batch, kv_heads, max_len, head_dim, block;
+} ml_kv8_cache;
+
+/*
+ * Appends up to `tokens` rows of k and v ([batch, kv_heads, tokens, head_dim]
+ * at element strides (batch, head, token), multiples of 8, head_dim
+ * contiguous) to each sequence: row t goes to position start[b] + t for t <
+ * counts[b] (counts NULL: all rows).  start / counts are int64 device arrays,
+ * read with stride 0 (one value for the batch) or 1.  Every block that gets a
+ * row is requantised from its unquantised rows: a = max |x| over the block,
+ * scale = a / qmax (qmax 127, e4m3 448), code = round(x * qmax / a), half to
+ * even; a block holding inf or NaN reads back as NaN.  Rows that would pass
+ * max_len, and sequences whose start is negative or past max_len, write
+ * nothing.  A start inside a block needs that block's earlier rows to be in
+ * the tail: they are after any append that ended in this block or the next.
+ * Positions past the last new row keep what they held.
+ */
+ML_API int ml_kv8_append(const ml_kv8_cache* cache, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, int64_t tokens,
+                         const int64_t* start, int64_t start_stride, const int64_t* counts,
+                         int64_t counts_stride, void* stream);
+
+/*
+ * Attention of `tokens` query rows per sequence over such a cache:
+ * out[b, t, h, :] = sum_j softmax_j(scale * q[b, h, t] . k_j) v_j over the
+ * positions j <= start[b] + t (clipped to max_len) of kv head h / (q_heads /
+ * kv_heads).  q is [batch, q_heads, tokens, head_dim] at element strides
+ * (batch, head, token), multiples of 8, head_dim contiguous; out [batch,
+ * tokens, q_heads, head_dim] contiguous; both in the cache's dtype.  Rows t >=
+ * counts[b], and rows that see no position, are zeros.  fp32 scores, softmax
+ * statistics and accumulation.  workspace >=
+ * ml_kv8_attention_workspace_bytes (0: may be NULL), 16-byte aligned, not
+ * shared with a call that may run at the same time.
+ */
+ML_API size_t ml_kv8_attention_workspace_bytes(const ml_kv8_cache* cache, int64_t q_heads,
+                                               int64_t tokens);
+ML_API int ml_kv8_attention(const ml_kv8_cache* cache, const void* q, const int64_t* q_strides,
+                            int64_t q_heads, int64_t tokens, const int64_t* start,
+                            int64_t start_stride, const int64_t* counts, int64_t counts_stride,
+                            float scale, void* out, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/*
+ * Samples one token from each row of logits [rows, vocab] (row pitch ld
+ * elements, any of the three dtypes) with temperature, top-k, top-p and min-p
+ * from uniform[row] in [0, 1) (values outside are clamped): tokens are ordered
+ * by logit, largest first, equal logits by index; of the first top_k (<= 0:
+ * all), the shortest prefix holding top_p of their weight exp(logit /
+ * temperature), of those the ones with at least min_p times the largest
+ * weight, never fewer than one; id = the first kept index, in vocabulary
+ * order, at which the running weight exceeds uniform times the kept weight;
+ * logprob = log of its share of the kept weight.  temperature <= 0 or NaN: the
+ * first token, logprob 0.  NaN and -inf logits are never taken; a row of
+ * nothing else gives id -1, logprob -inf.  Each of the four parameters is a
+ * device array [rows], or NULL and a value for all rows.  vocab <= 2^20.  The
+ * result does not depend on rows or on how the work is split.  No reference
+ * counterpart (the reference divides by the temperature and draws with
+ * torch.multinomial, generation.py:118-123; top_p only selects the rule).
+ */
+ML_API int ml_sample(const void* logits, int64_t ld, int logits_dtype, int64_t rows, int64_t vocab,
+                     const float* uniform, const float* temperature, float temperature_value,
+                     const int64_t* top_k, int64_t top_k_value, const float* top_p,
+                     float top_p_value, const float* min_p, float min_p_value, int64_t* id,
+                     float* logprob, void* stream);
+
+/*
  * Self-test of the bounded device-side waits (no reference counterpart):
  * enqueues on `stream` a one-warp kernel whose mbarrier wait can never
  * complete, bounded to limit_us (1,000 - 1,000,000 us); the wait gives up and

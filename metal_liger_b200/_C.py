@@ -63,6 +63,15 @@ class LoraProj(ctypes.Structure):
                 ("b_dtype", c_int), ("out_features", c_int64), ("scaling", c_float)]
 
 
+class Kv8Cache(ctypes.Structure):
+    """Mirror of ``ml_kv8_cache``."""
+
+    _fields_ = [("k_codes", c_void_p), ("v_codes", c_void_p), ("k_scale", c_void_p),
+                ("v_scale", c_void_p), ("k_tail", c_void_p), ("v_tail", c_void_p),
+                ("format", c_int), ("dtype", c_int), ("batch", c_int64), ("kv_heads", c_int64),
+                ("max_len", c_int64), ("head_dim", c_int64), ("block", c_int64)]
+
+
 # name -> (restype, argtypes).  Kept in the same order as the header.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ml_version": (c_int, []),
@@ -187,6 +196,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                      c_int64, c_int64, c_int64, c_int64, ctypes.POINTER(LoraProj),
                                      c_void_p, c_void_p, ctypes.POINTER(c_void_p),
                                      ctypes.POINTER(c_void_p), c_void_p, c_size_t, c_void_p]),
+    "ml_kv8_append": (c_int, [ctypes.POINTER(Kv8Cache), c_void_p, ctypes.POINTER(c_int64), c_void_p,
+                              ctypes.POINTER(c_int64), c_int64, c_void_p, c_int64, c_void_p,
+                              c_int64, c_void_p]),
+    "ml_kv8_attention_workspace_bytes": (c_size_t, [ctypes.POINTER(Kv8Cache), c_int64, c_int64]),
+    "ml_kv8_attention": (c_int, [ctypes.POINTER(Kv8Cache), c_void_p, ctypes.POINTER(c_int64),
+                                 c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_float,
+                                 c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ml_sample": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_float,
+                          c_void_p, c_int64, c_void_p, c_float, c_void_p, c_float, c_void_p,
+                          c_void_p, c_void_p]),
     "ml_device_error": (c_int, [c_void_p]),
 }
 

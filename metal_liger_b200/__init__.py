@@ -34,6 +34,13 @@ from metal_liger_b200.ops.fused_lora import (  # noqa: E402
     apply_fused_lora_linear,
     patch_fused_lora,
 )
+from metal_liger_b200.ops.quantized_kv import (  # noqa: E402
+    QuantizedKV,
+    allocate_quantized_kv,
+    quantized_kv_append,
+    quantized_kv_attention,
+)
+from metal_liger_b200.ops.fused_sampling import fused_sample  # noqa: E402
 from metal_liger_b200.patch import apply_metal_liger_to_qwen3vl  # noqa: E402
 from metal_liger_b200._compile import apply_compile  # noqa: E402
 
@@ -47,6 +54,11 @@ __all__ = [
     "apply_fused_lora_mlp",
     "apply_fused_lora_linear",
     "patch_fused_lora",
+    "QuantizedKV",
+    "allocate_quantized_kv",
+    "quantized_kv_append",
+    "quantized_kv_attention",
+    "fused_sample",
     "apply_compile",
     "register_metal_liger_ops",
     "install_as_metal_liger",

@@ -973,7 +973,178 @@ def decode_qk_attention_cuda(q: Tensor, k: Tensor, v: Tensor, wq: Tensor, wk: Te
     return out
 
 
+# ---------------------------------------------------------------------------
+# 8-bit KV cache and sampling
+# ---------------------------------------------------------------------------
+
+_KV8_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_KV8_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def _on_device(t: Tensor):
+    """A guard that makes ``t``'s device current: a kernel is launched on the
+    current one, whatever its stream's.  None where it is current already."""
+    if t.device.index == torch.cuda.current_device():
+        return None
+    return torch.cuda.device(t.device)
+
+
+def _kv8_cache(name: str, kc: Tensor, vc: Tensor, ks: Tensor, vs: Tensor, kt: Tensor, vt: Tensor,
+               dtype: torch.dtype) -> _C.Kv8Cache:
+    """The checked C description of a quantised cache."""
+    if kc.dim() != 4 or ks.dim() != 3 or kt.dim() != 5:
+        raise RuntimeError(f"{name}: codes must be [B, Hkv, L, D], scales [B, Hkv, L / block] and "
+                           f"tails [B, Hkv, 2, block, D]")
+    fmt = _KV8_FORMATS.get(kc.dtype)
+    if fmt is None or vc.dtype != kc.dtype:
+        raise RuntimeError(f"{name}: codes are int8 or float8_e4m3fn, K and V alike, not "
+                           f"{kc.dtype} / {vc.dtype}")
+    if dtype not in _KV8_DTYPES or kt.dtype != dtype or vt.dtype != dtype:
+        raise RuntimeError(f"{name}: bf16 or fp16 rows and tails of the same dtype, not {dtype} / "
+                           f"{kt.dtype}")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise RuntimeError(f"{name}: scales are float32")
+    B, H, L, D = kc.shape
+    block = kt.shape[3]
+    if vc.shape != kc.shape or vs.shape != ks.shape or vt.shape != kt.shape or block == 0 or \
+            L % block or ks.shape != (B, H, L // block) or kt.shape != (B, H, 2, block, D):
+        raise RuntimeError(f"{name}: cache shapes do not match: codes {tuple(kc.shape)}, scales "
+                           f"{tuple(ks.shape)}, tails {tuple(kt.shape)}")
+    for t in (kc, vc, ks, vs, kt, vt):
+        if not t.is_contiguous():
+            raise RuntimeError(f"{name}: cache buffers must be contiguous")
+    return _C.Kv8Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(),
+                       vt.data_ptr(), fmt, _C.DTYPE_CODES[dtype], B, H, L, D, block)
+
+
+def _kv8_rows(t: Tensor):
+    """(tensor, element strides of its first three dimensions) of [B, H, T, D]
+    rows the kernels can read in 16-byte vectors in place, else of a copy."""
+    st = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+    if t.stride(3) != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = t.stride()[:3]
+    return t, (ctypes.c_int64 * 3)(*st)
+
+
+def _kv8_index(name: str, what: str, t: Tensor | None, batch: int):
+    """(pointer, stride) of an int64 [B], [1] or 0-d device tensor."""
+    if t is None:
+        return None, 0
+    n = t.numel()
+    if t.dtype != torch.int64 or n not in (1, batch) or t.dim() > 1:
+        raise RuntimeError(f"{name}: {what} must be an int64 tensor of 1 or {batch} values, not "
+                           f"{t.dtype} {tuple(t.shape)}")
+    if n > 1 and t.stride(0) != 1:
+        raise RuntimeError(f"{name}: {what} must be contiguous")
+    return t.data_ptr(), 1 if n > 1 else 0
+
+
+def kv8_append_cuda(k: Tensor, v: Tensor, start: Tensor, counts: Tensor | None, k_codes: Tensor,
+                    v_codes: Tensor, k_scale: Tensor, v_scale: Tensor, k_tail: Tensor,
+                    v_tail: Tensor) -> None:
+    """Append k, v [B, Hkv, T, D] (bf16 or fp16) at positions ``start`` + t of
+    each sequence (rows t >= ``counts`` are padding) to a cache held in 8
+    bits, in place."""
+    name = "kv8_append"
+    _C.require_cuda(name, k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)
+    c = _kv8_cache(name, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail, k.dtype)
+    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or \
+            (k.shape[0], k.shape[1], k.shape[3]) != (c.batch, c.kv_heads, c.head_dim):
+        raise RuntimeError(f"{name}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match the "
+                           f"cache {tuple(k_codes.shape)}")
+    sp, ss = _kv8_index(name, "start", start, c.batch)
+    cp, cs = _kv8_index(name, "counts", counts, c.batch)
+    guard = _on_device(k)
+    if guard is not None:
+        with guard:
+            return kv8_append_cuda(k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail,
+                                   v_tail)
+    (k, kst), (v, vst) = _kv8_rows(k), _kv8_rows(v)
+    _C.call("ml_kv8_append", ctypes.byref(c), k.data_ptr(), kst, v.data_ptr(), vst, k.shape[2], sp,
+            ss, cp, cs, _C.stream_of(k))
+
+
+def kv8_attention_cuda(q: Tensor, start: Tensor, counts: Tensor | None, k_codes: Tensor,
+                       v_codes: Tensor, k_scale: Tensor, v_scale: Tensor, k_tail: Tensor,
+                       v_tail: Tensor, scale: float) -> Tensor:
+    """Attention of q [B, Hq, T, D] over the positions <= ``start`` + t of a
+    cache held in 8 bits; returns [B, T, Hq, D] in q's dtype."""
+    name = "kv8_attention"
+    _C.require_cuda(name, q, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)
+    c = _kv8_cache(name, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail, q.dtype)
+    if q.dim() != 4 or q.shape[0] != c.batch or q.shape[3] != c.head_dim or \
+            q.shape[1] == 0 or q.shape[1] % c.kv_heads:
+        raise RuntimeError(f"{name}: q {tuple(q.shape)} does not match the cache "
+                           f"{tuple(k_codes.shape)}")
+    sp, ss = _kv8_index(name, "start", start, c.batch)
+    cp, cs = _kv8_index(name, "counts", counts, c.batch)
+    guard = _on_device(q)
+    if guard is not None:
+        with guard:
+            return kv8_attention_cuda(q, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail,
+                                      v_tail, scale)
+    B, Hq, T, D = q.shape
+    q, st = _kv8_rows(q)
+    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    nbytes = _C.load().ml_kv8_attention_workspace_bytes(ctypes.byref(c), Hq, T)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _C.call("ml_kv8_attention", ctypes.byref(c), q.data_ptr(), st, Hq, T, sp, ss, cp, cs,
+            float(scale), out.data_ptr(), _C.ptr(ws), nbytes, _C.stream_of(q))
+    return out
+
+
+def _sample_param(what: str, t: Tensor | None, rows: int, dtype: torch.dtype):
+    if t is None:
+        return None, None
+    if t.dim() != 1 or t.shape[0] != rows:
+        raise RuntimeError(f"sample: {what} must have {rows} values, not {tuple(t.shape)}")
+    if t.dtype != dtype or not t.is_contiguous():
+        t = t.to(dtype).contiguous()
+    return t, t.data_ptr()
+
+
+def sample_cuda(logits: Tensor, uniform: Tensor, temperature: Tensor | None,
+                temperature_value: float, top_k: Tensor | None, top_k_value: int,
+                top_p: Tensor | None, top_p_value: float, min_p: Tensor | None,
+                min_p_value: float):
+    """(id int64 [B], logprob fp32 [B]) of one token per row of logits [B, V]
+    from uniform [B]; each parameter a [B] tensor or, without one, a value."""
+    _C.require_cuda("sample", logits, uniform, temperature, top_k, top_p, min_p)
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise RuntimeError(f"sample: logits must be [B, V], not {tuple(logits.shape)}")
+    guard = _on_device(logits)
+    if guard is not None:
+        with guard:
+            return sample_cuda(logits, uniform, temperature, temperature_value, top_k,
+                               top_k_value, top_p, top_p_value, min_p, min_p_value)
+    B, V = logits.shape
+    code = _C.dtype_code(logits)
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    uniform, up = _sample_param("uniform", uniform, B, torch.float32)
+    temperature, tp = _sample_param("temperature", temperature, B, torch.float32)
+    top_k, kp = _sample_param("top_k", top_k, B, torch.int64)
+    top_p, pp = _sample_param("top_p", top_p, B, torch.float32)
+    min_p, mp = _sample_param("min_p", min_p, B, torch.float32)
+    index = torch.empty(B, dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(B, dtype=torch.float32, device=logits.device)
+    _C.call("ml_sample", logits.data_ptr(), logits.stride(0), code, B, V, up, tp,
+            float(temperature_value), kp, int(top_k_value), pp, float(top_p_value), mp,
+            float(min_p_value), index.data_ptr(), logprob.data_ptr(), _C.stream_of(logits))
+    return index, logprob
+
+
 _SCHEMAS = {
+    "kv8_append": "kv8_append(Tensor k, Tensor v, Tensor start, Tensor? counts, "
+                  "Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scale, "
+                  "Tensor(d!) v_scale, Tensor(e!) k_tail, Tensor(f!) v_tail) -> ()",
+    "kv8_attention": "kv8_attention(Tensor q, Tensor start, Tensor? counts, Tensor k_codes, "
+                     "Tensor v_codes, Tensor k_scale, Tensor v_scale, Tensor k_tail, "
+                     "Tensor v_tail, float scale) -> Tensor",
+    "sample": "sample(Tensor logits, Tensor uniform, Tensor? temperature, "
+              "float temperature_value, Tensor? top_k, int top_k_value, Tensor? top_p, "
+              "float top_p_value, Tensor? min_p, float min_p_value) -> (Tensor, Tensor)",
     "decode_qk_norm_rope": "decode_qk_norm_rope(Tensor q, Tensor k, Tensor v, Tensor wq, "
                            "Tensor wk, float eps_q, float eps_k, Tensor cos, Tensor sin, "
                            "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor pos) -> Tensor",
@@ -1034,6 +1205,9 @@ _SCHEMAS = {
 }
 
 _CUDA_IMPLS = {
+    "kv8_append": kv8_append_cuda,
+    "kv8_attention": kv8_attention_cuda,
+    "sample": sample_cuda,
     "decode_qk_norm_rope": decode_qk_norm_rope_cuda,
     "decode_attention": decode_attention_cuda,
     "gemv_multi": gemv_multi_cuda,
@@ -1187,7 +1361,24 @@ def _fake_impls():
         B, Hkv, L, D = k_cache.shape
         return torch.empty((B, q.numel() // (B * D), 1, D), dtype=q.dtype, device=q.device)
 
+    def kv8_append_fake(k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail):
+        return None
+
+    def kv8_attention_fake(q, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail,
+                           scale):
+        B, Hq, T, D = q.shape
+        return torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+
+    def sample_fake(logits, uniform, temperature, temperature_value, top_k, top_k_value, top_p,
+                    top_p_value, min_p, min_p_value):
+        B = logits.shape[0]
+        return (torch.empty(B, dtype=torch.int64, device=logits.device),
+                torch.empty(B, dtype=torch.float32, device=logits.device))
+
     return {
+        "kv8_append": kv8_append_fake,
+        "kv8_attention": kv8_attention_fake,
+        "sample": sample_fake,
         "decode_qk_norm_rope": decode_qk_fake,
         "decode_attention": decode_attention_fake,
         "gemv_multi": gemv_multi_fake,

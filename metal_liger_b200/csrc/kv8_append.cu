@@ -1,0 +1,230 @@
+// Appending K and V rows to a KV cache held in 8 bits.
+//
+// A block of `block` consecutive positions of one kv head has one fp32 scale.
+// With a = max |x| over the block's live values x,
+//   scale = a / qmax,   code = round(x * qmax / a)      (qmax: 127, or 448 for e4m3)
+// rounded half to even to an integer, or to the nearest e4m3 value.  x has at
+// most 11 significant bits and qmax 7, so x * qmax is exact in fp32, the one
+// IEEE division is correctly rounded, and its quotient is a tie exactly where
+// the true quotient is one (two such ratios that differ do so by more than
+// 2^-22 of their size): every code is the one the formula gives in exact
+// arithmetic.  A block without a non-zero value has scale 0 and codes 0; a
+// block holding an infinity or NaN gets that as its scale and codes 0, so it
+// reads back as NaN.
+//
+// Each block is quantised from the values themselves, never from codes: the
+// rows of the last two blocks written are also kept unquantised (`tail`, slot
+// block & 1), and a call that continues a partly filled block takes its older
+// rows from there.  The cache after any sequence of calls is therefore the
+// cache after one call with all the rows.  Two slots, not one, so that a
+// sequence can be taken back across a block border.
+//
+// A CTA takes one block of one kv head, K or V: its rows (new ones from the
+// call, older ones from the tail) go to registers as 16-byte vectors, one
+// block-wide maximum of |bits| (for bf16 and fp16 the order of the magnitudes
+// with inf and NaN on top), then the codes.  Rows past the last new one are
+// left as they were.  Memory bound: 2 bytes read and 1 written per element.
+#include "kv8.cuh"
+
+#include <cuda_fp8.h>
+
+namespace ml {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendArgs {
+  const void* src[2];       // k, v [B, Hkv, T, D] at element strides
+  int64_t stride[2][3];     // batch, head, token
+  uint8_t* codes[2];        // [B, Hkv, L, D]
+  float* scale[2];          // [B, Hkv, L / block]
+  void* tail[2];            // [B, Hkv, 2, block, D]
+  Kv8Span span;
+  int heads, max_len, block;
+};
+
+template <typename T>
+__device__ __forceinline__ float unpack(uint32_t w, int half) {
+  T v;
+  const uint16_t u = (uint16_t)(half ? w >> 16 : w);
+  memcpy(&v, &u, 2);
+  return to_f32(v);
+}
+
+// Eight codes of a 16-byte vector; `mul` = qmax (times a power of two that
+// keeps x * qmax finite), `top` = a (times the same).
+template <typename T, int FMT>
+__device__ __forceinline__ uint2 quantise8(const uint4& x, float mul, float top) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t out[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = __fdiv_rn(unpack<T>(w[i], 0) * mul, top);
+    const float b = __fdiv_rn(unpack<T>(w[i], 1) * mul, top);
+    uint32_t two;
+    if (FMT == ML_KV8_INT8) {
+      two = (uint32_t)(uint8_t)(int8_t)__float2int_rn(a) |
+            ((uint32_t)(uint8_t)(int8_t)__float2int_rn(b) << 8);
+    } else {
+      two = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    }
+    out[i >> 1] |= two << (16 * (i & 1));
+  }
+  return make_uint2(out[0], out[1]);
+}
+
+// Block `blk` of (b, h): rows [start, end) are new, older ones of the block
+// come from the tail.  NV 16-byte vectors per thread cover the block.
+template <typename T, int FMT, int D, int NV>
+__device__ __forceinline__ void append_block(const AppendArgs& a, int which, int b, int h,
+                                             int64_t blk, int64_t start, int64_t end, bool keep,
+                                             uint32_t* red) {
+  constexpr int VPR = D / 8;  // vectors per row
+  const int64_t base = blk * a.block;
+  const int live = (int)min((int64_t)a.block, end - base);
+  const int64_t bh = (int64_t)b * a.heads + h;
+  const T* src = static_cast<const T*>(a.src[which]) + b * a.stride[which][0] +
+                 h * a.stride[which][1];
+  T* tail = static_cast<T*>(a.tail[which]) + (bh * 2 + (blk & 1)) * a.block * D;
+  uint4 x[NV];
+  uint32_t top2 = 0;  // |bits| maxima of even and odd elements
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = i * kThreads + threadIdx.x;
+    const int row = v / VPR, col = (v % VPR) * 8;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (row < live) {
+      const int64_t p = base + row;
+      const T* from = p < start ? tail + row * D + col : src + (p - start) * a.stride[which][2] + col;
+      x[i] = *reinterpret_cast<const uint4*>(from);
+    }
+    top2 = __vmaxu2(top2, x[i].x & 0x7fff7fffu);
+    top2 = __vmaxu2(top2, x[i].y & 0x7fff7fffu);
+    top2 = __vmaxu2(top2, x[i].z & 0x7fff7fffu);
+    top2 = __vmaxu2(top2, x[i].w & 0x7fff7fffu);
+  }
+  uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  __syncthreads();  // `red` may still be read by an earlier block of this CTA
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) top = max(top, red[i]);
+  constexpr float qmax = FMT == ML_KV8_INT8 ? 127.f : 448.f;
+  const float amax = unpack<T>(top, 0);
+  if (threadIdx.x == 0) a.scale[which][bh * (a.max_len / a.block) + blk] = __fdiv_rn(amax, qmax);
+  const bool finite = amax <= 3.4028235e38f && amax > 0.f;
+  // x * qmax has to stay finite: values near the top of bf16 are halved 16
+  // times on both sides of the division first (exact)
+  const float down = amax > 1e30f ? 1.52587890625e-5f : 1.f;
+  uint8_t* codes = a.codes[which] + (bh * a.max_len + base) * D;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = i * kThreads + threadIdx.x;
+    const int row = v / VPR, col = (v % VPR) * 8;
+    if (row >= live) continue;
+    uint2 q = make_uint2(0, 0);
+    if (finite) q = quantise8<T, FMT>(x[i], qmax * down, amax * down);
+    *reinterpret_cast<uint2*>(codes + (int64_t)row * D + col) = q;
+    if (keep && base + row >= start) *reinterpret_cast<uint4*>(tail + row * D + col) = x[i];
+  }
+}
+
+// Grid (blocks a call can touch, kv heads x {K, V}, batch).
+template <typename T, int FMT, int D, int NV>
+__global__ void __launch_bounds__(kThreads)
+kv8_append_kernel(const __grid_constant__ AppendArgs a) {
+  __shared__ uint32_t red[kThreads / 32];
+  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1;
+  const int64_t start = a.span.first(b);
+  if (start < 0 || start >= a.max_len) return;
+  const int64_t end = min((int64_t)a.max_len, start + a.span.count(b));
+  const int64_t first = start / a.block, last = (end - 1) / a.block;
+  const int64_t blk = first + blockIdx.x;
+  if (end <= start || blk > last) return;
+  // The block that replaces the tail slot the first block still reads (the
+  // last or the one before, of the first one's parity) is done by the same
+  // CTA after it.
+  int64_t after = -1;
+  if (start % a.block != 0 && last - first >= 2) after = (last - first) % 2 == 0 ? last : last - 1;
+  if (blk == after) return;
+  append_block<T, FMT, D, NV>(a, which, b, h, blk, start, end, blk >= last - 1, red);
+  if (blk == first && after >= 0) {
+    __syncthreads();  // every thread has its tail rows
+    append_block<T, FMT, D, NV>(a, which, b, h, after, start, end, true, red);
+  }
+}
+
+template <typename T, int FMT, int D>
+int launch_append(const AppendArgs& a, dim3 grid, cudaStream_t st) {
+  switch (a.block * (D / 8) / kThreads) {
+#define ML_KV8_NV(NV_) \
+  case NV_: kv8_append_kernel<T, FMT, D, NV_><<<grid, kThreads, 0, st>>>(a); break;
+    ML_KV8_NV(1) ML_KV8_NV(2) ML_KV8_NV(4) ML_KV8_NV(8) ML_KV8_NV(16)
+#undef ML_KV8_NV
+    default: set_error("kv8_append: unsupported block size"); return ML_ERR_INVALID_ARG;
+  }
+  ML_CHECK_LAUNCH("kv8_append");
+  return ML_OK;
+}
+
+template <typename T, int FMT>
+int launch_append_dim(const AppendArgs& a, int64_t dim, dim3 grid, cudaStream_t st) {
+  if (dim == 64) return launch_append<T, FMT, 64>(a, grid, st);
+  if (dim == 128) return launch_append<T, FMT, 128>(a, grid, st);
+  return launch_append<T, FMT, 256>(a, grid, st);
+}
+
+}  // namespace
+}  // namespace ml
+
+using namespace ml;
+
+extern "C" int ml_kv8_append(const ml_kv8_cache* cache, const void* k, const int64_t* k_strides,
+                             const void* v, const int64_t* v_strides, int64_t tokens,
+                             const int64_t* start, int64_t start_stride, const int64_t* counts,
+                             int64_t counts_stride, void* stream) {
+  int rc = kv8_check("kv8_append", cache);
+  if (rc != ML_OK) return rc;
+  ML_CHECK_ARG(tokens >= 0 && tokens < ((int64_t)1 << 30), "kv8_append: bad token count");
+  if (cache->batch == 0 || tokens == 0) return ML_OK;
+  ML_CHECK_ARG(k && v && start && k_strides && v_strides && cache->k_tail && cache->v_tail,
+               "kv8_append: null pointer");
+  ML_CHECK_ARG((start_stride == 0 || start_stride == 1) &&
+                   (counts_stride == 0 || counts_stride == 1),
+               "kv8_append: start / counts strides are 0 or 1");
+  ML_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(cache->k_tail) && aligned16(cache->v_tail),
+               "kv8_append: k, v and tail must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    ML_CHECK_ARG(k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0,
+                 "kv8_append: k and v strides must be multiples of 8 elements");
+  AppendArgs a;
+  a.src[0] = k;
+  a.src[1] = v;
+  for (int i = 0; i < 3; ++i) {
+    a.stride[0][i] = k_strides[i];
+    a.stride[1][i] = v_strides[i];
+  }
+  a.codes[0] = static_cast<uint8_t*>(cache->k_codes);
+  a.codes[1] = static_cast<uint8_t*>(cache->v_codes);
+  a.scale[0] = cache->k_scale;
+  a.scale[1] = cache->v_scale;
+  a.tail[0] = cache->k_tail;
+  a.tail[1] = cache->v_tail;
+  a.span = {start, start_stride, counts, counts_stride, (int)tokens};
+  a.heads = (int)cache->kv_heads;
+  a.max_len = (int)cache->max_len;
+  a.block = (int)cache->block;
+  // an unaligned start can touch one block more than the rows fill
+  const int64_t nblk = (tokens + cache->block - 2) / cache->block + 1;
+  const int64_t most = cache->max_len / cache->block;
+  const dim3 grid((unsigned)(nblk < most ? nblk : most), (unsigned)(2 * cache->kv_heads),
+                  (unsigned)cache->batch);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool bf = cache->dtype == ML_DTYPE_BF16;
+  if (cache->format == ML_KV8_INT8)
+    return bf ? launch_append_dim<__nv_bfloat16, ML_KV8_INT8>(a, cache->head_dim, grid, st)
+              : launch_append_dim<__half, ML_KV8_INT8>(a, cache->head_dim, grid, st);
+  return bf ? launch_append_dim<__nv_bfloat16, ML_KV8_E4M3>(a, cache->head_dim, grid, st)
+            : launch_append_dim<__half, ML_KV8_E4M3>(a, cache->head_dim, grid, st);
+}

@@ -1,0 +1,125 @@
+"""A KV cache held in 8 bits: its buffers, the append and the attention over it.
+
+No counterpart in the reference, whose static cache keeps the model's dtype
+(generation.py:18-66).  One layer's cache is a ``QuantizedKV`` of six device
+buffers: int8 or e4m3 codes for K and V, one fp32 scale for each block of
+positions and kv head, and the unquantised rows of the last two blocks (the
+"tail"), so that a block is always quantised from its values themselves:
+
+    a = max |x| over the block,   scale = a / qmax,   code = round(x * qmax / a)
+
+with qmax 127 (int8) or 448 (e4m3), rounded half to even.  It halves the bytes
+a decode step reads per position and the memory per sequence.
+
+    kv = allocate_quantized_kv(batch, kv_heads, max_len, head_dim, "int8")
+    quantized_kv_append(kv, k, v, start)              # in place, start on the device
+    out = quantized_kv_attention(q, kv, start)        # [B, T, Hq, D]
+
+``start`` (int64, one value or one per sequence) is the number of positions a
+sequence held before the step, the same for the append and the attention;
+neither advances it.  It stays on the device, so a captured CUDA graph of the
+step follows it.
+"""
+
+from typing import NamedTuple, Optional
+
+import torch
+from torch import Tensor
+
+from metal_liger_b200 import _torch_library as _tl
+
+CACHE_DTYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+DEFAULT_BLOCK = 64
+
+
+class QuantizedKV(NamedTuple):
+    """One layer's cache buffers."""
+
+    k_codes: Tensor   # [B, Hkv, L, D] int8 or float8_e4m3fn
+    k_scale: Tensor   # [B, Hkv, L / block] float32
+    k_tail: Tensor    # [B, Hkv, 2, block, D] bf16 or fp16
+    v_codes: Tensor
+    v_scale: Tensor
+    v_tail: Tensor
+
+    @property
+    def max_len(self) -> int:
+        return self.k_codes.shape[2]
+
+    @property
+    def block(self) -> int:
+        return self.k_tail.shape[3]
+
+    def dequantize(self):
+        """(K, V) [B, Hkv, L, D] in the tails' dtype: code * scale, rounded once."""
+        return tuple(
+            (c.float().view(*s.shape, -1) * s[..., None]).view(c.shape).to(t.dtype)
+            for c, s, t in ((self.k_codes, self.k_scale, self.k_tail),
+                            (self.v_codes, self.v_scale, self.v_tail)))
+
+
+def allocate_quantized_kv(batch: int, kv_heads: int, max_len: int, head_dim: int,
+                          cache_dtype: str = "int8", dtype: torch.dtype = torch.bfloat16,
+                          block: int = DEFAULT_BLOCK, device="cuda") -> QuantizedKV:
+    """Zeroed buffers for ``max_len`` positions (rounded up to whole blocks).
+
+    ``cache_dtype`` "int8" or "fp8" (e4m3), ``dtype`` (bf16 or fp16) that of the
+    rows appended and of the queries, ``head_dim`` 64, 128 or 256, ``block`` 32,
+    64 or 128 positions per scale."""
+    if cache_dtype not in CACHE_DTYPES:
+        raise ValueError(f"cache_dtype {cache_dtype!r}: one of {sorted(CACHE_DTYPES)}")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"dtype {dtype}: bfloat16 or float16")
+    if head_dim not in (64, 128, 256) or block not in (32, 64, 128):
+        raise ValueError(f"head_dim {head_dim} (64, 128 or 256), block {block} (32, 64 or 128)")
+    if batch < 1 or kv_heads < 1 or max_len < 1:
+        raise ValueError("batch, kv_heads and max_len are at least 1")
+    length = -(-max_len // block) * block
+    shape = (batch, kv_heads)
+
+    def half():
+        return (torch.zeros((*shape, length, head_dim), dtype=torch.int8,
+                            device=device).view(CACHE_DTYPES[cache_dtype]),
+                torch.zeros((*shape, length // block), dtype=torch.float32, device=device),
+                torch.zeros((*shape, 2, block, head_dim), dtype=dtype, device=device))
+
+    return QuantizedKV(*half(), *half())
+
+
+def _eager(t: Tensor) -> bool:
+    return t.is_cuda and type(t) is Tensor and not torch.compiler.is_compiling()
+
+
+def quantized_kv_append(kv: QuantizedKV, k: Tensor, v: Tensor, start: Tensor,
+                        counts: Optional[Tensor] = None) -> None:
+    """Write k, v [B, Hkv, T, D] (any strides) at positions ``start`` + t, in place.
+
+    ``counts`` (int64): how many of the T rows are real in each sequence, the
+    others being padding.  Blocks that get a row are requantised whole; rows
+    past ``max_len`` are dropped, as are those of a sequence whose start is
+    negative; positions past the last new one keep what they held.
+
+    ``start`` may go back (a drafted continuation rejected, a new prompt at 0):
+    to any block border, or into a block that is the last one written or the
+    one before it, whose unquantised rows the tail still has."""
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise RuntimeError("quantized_kv_append has no backward: call it under torch.no_grad()")
+    op = _tl.kv8_append_cuda if _eager(k) else torch.ops.metal_liger.kv8_append
+    op(k, v, start, counts, kv.k_codes, kv.v_codes, kv.k_scale, kv.v_scale, kv.k_tail, kv.v_tail)
+
+
+def quantized_kv_attention(q: Tensor, kv: QuantizedKV, start: Tensor,
+                           counts: Optional[Tensor] = None,
+                           scale: Optional[float] = None) -> Tensor:
+    """softmax(scale * q k^T) v of q [B, Hq, T, D] over the cache, [B, T, Hq, D].
+
+    Query t of a sequence sees positions j <= ``start`` + t, so the call follows
+    the append of the same tokens; Hq is a multiple of the cache's kv heads.
+    Rows t >= ``counts`` and rows that see nothing are zeros.  ``scale``
+    defaults to D ** -0.5."""
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError("quantized_kv_attention has no backward: call it under "
+                           "torch.no_grad()")
+    op = _tl.kv8_attention_cuda if _eager(q) else torch.ops.metal_liger.kv8_attention
+    return op(q, start, counts, kv.k_codes, kv.v_codes, kv.k_scale, kv.v_scale, kv.k_tail,
+              kv.v_tail, q.shape[-1] ** -0.5 if scale is None else scale)

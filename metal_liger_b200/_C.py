@@ -269,6 +269,20 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def raw_stream(device: int) -> int:
+    """``stream_of`` for a device index."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: int):
+    """Makes ``device`` current for a block: a kernel is launched on the current
+    device, whatever its stream's."""
+    return _HERE if torch._C._cuda_getDevice() == device else torch.cuda.device(device)
+
+
 def require_cuda(name: str, *tensors: torch.Tensor | None) -> None:
     dev = None
     for t in tensors:

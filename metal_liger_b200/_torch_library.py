@@ -981,12 +981,12 @@ _KV8_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _KV8_DTYPES = (torch.bfloat16, torch.float16)
 
 
-def _on_device(t: Tensor):
-    """A guard that makes ``t``'s device current: a kernel is launched on the
-    current one, whatever its stream's.  None where it is current already."""
-    if t.device.index == torch.cuda.current_device():
-        return None
-    return torch.cuda.device(t.device)
+def _same_device(name: str, first: Tensor, *rest: Tensor | None) -> int:
+    """The CUDA device index all tensors are on (raises where they are not)."""
+    dev = first.get_device()
+    if dev < 0 or any(t is not None and t.get_device() != dev for t in rest):
+        _C.require_cuda(name, first, *rest)
+    return dev
 
 
 def _kv8_cache(name: str, kc: Tensor, vc: Tensor, ks: Tensor, vs: Tensor, kt: Tensor, vt: Tensor,
@@ -1004,27 +1004,34 @@ def _kv8_cache(name: str, kc: Tensor, vc: Tensor, ks: Tensor, vs: Tensor, kt: Te
                            f"{kt.dtype}")
     if ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise RuntimeError(f"{name}: scales are float32")
-    B, H, L, D = kc.shape
-    block = kt.shape[3]
-    if vc.shape != kc.shape or vs.shape != ks.shape or vt.shape != kt.shape or block == 0 or \
-            L % block or ks.shape != (B, H, L // block) or kt.shape != (B, H, 2, block, D):
+    shape, tail = kc.shape, kt.shape
+    B, H, L, D = shape
+    block = tail[3]
+    if vc.shape != shape or vt.shape != tail or block == 0 or L % block or \
+            tail != (B, H, 2, block, D) or ks.shape != (B, H, L // block) or vs.shape != ks.shape:
         raise RuntimeError(f"{name}: cache shapes do not match: codes {tuple(kc.shape)}, scales "
                            f"{tuple(ks.shape)}, tails {tuple(kt.shape)}")
-    for t in (kc, vc, ks, vs, kt, vt):
-        if not t.is_contiguous():
-            raise RuntimeError(f"{name}: cache buffers must be contiguous")
+    if not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous()
+            and vs.is_contiguous() and kt.is_contiguous() and vt.is_contiguous()):
+        raise RuntimeError(f"{name}: cache buffers must be contiguous")
     return _C.Kv8Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(),
                        vt.data_ptr(), fmt, _C.DTYPE_CODES[dtype], B, H, L, D, block)
+
+
+_Strides = ctypes.c_int64 * 3
 
 
 def _kv8_rows(t: Tensor):
     """(tensor, element strides of its first three dimensions) of [B, H, T, D]
     rows the kernels can read in 16-byte vectors in place, else of a copy."""
-    st = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
-    if t.stride(3) != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        st = t.stride()[:3]
-    return t, (ctypes.c_int64 * 3)(*st)
+    b, h, r, d = t.stride()
+    if d != 1 or (b | h | r) & 7 or t.data_ptr() & 15:
+        n = t.shape
+        b, h, r = (0 if n[0] == 1 else b, 0 if n[1] == 1 else h, 0 if n[2] == 1 else r)
+        if d != 1 or (b | h | r) & 7 or t.data_ptr() & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+            b, h, r, _ = t.stride()
+    return t, _Strides(b, h, r)
 
 
 def _kv8_index(name: str, what: str, t: Tensor | None, batch: int):
@@ -1032,10 +1039,10 @@ def _kv8_index(name: str, what: str, t: Tensor | None, batch: int):
     if t is None:
         return None, 0
     n = t.numel()
-    if t.dtype != torch.int64 or n not in (1, batch) or t.dim() > 1:
+    if t.dtype != torch.int64 or (n != 1 and n != batch) or t.dim() > 1:
         raise RuntimeError(f"{name}: {what} must be an int64 tensor of 1 or {batch} values, not "
                            f"{t.dtype} {tuple(t.shape)}")
-    if n > 1 and t.stride(0) != 1:
+    if n > 1 and not t.is_contiguous():
         raise RuntimeError(f"{name}: {what} must be contiguous")
     return t.data_ptr(), 1 if n > 1 else 0
 
@@ -1047,22 +1054,20 @@ def kv8_append_cuda(k: Tensor, v: Tensor, start: Tensor, counts: Tensor | None, 
     each sequence (rows t >= ``counts`` are padding) to a cache held in 8
     bits, in place."""
     name = "kv8_append"
-    _C.require_cuda(name, k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)
+    dev = _same_device(name, k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail,
+                       v_tail)
     c = _kv8_cache(name, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail, k.dtype)
-    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or \
-            (k.shape[0], k.shape[1], k.shape[3]) != (c.batch, c.kv_heads, c.head_dim):
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or shape[0] != c.batch or \
+            shape[1] != c.kv_heads or shape[3] != c.head_dim:
         raise RuntimeError(f"{name}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match the "
                            f"cache {tuple(k_codes.shape)}")
-    sp, ss = _kv8_index(name, "start", start, c.batch)
-    cp, cs = _kv8_index(name, "counts", counts, c.batch)
-    guard = _on_device(k)
-    if guard is not None:
-        with guard:
-            return kv8_append_cuda(k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail,
-                                   v_tail)
-    (k, kst), (v, vst) = _kv8_rows(k), _kv8_rows(v)
-    _C.call("ml_kv8_append", ctypes.byref(c), k.data_ptr(), kst, v.data_ptr(), vst, k.shape[2], sp,
-            ss, cp, cs, _C.stream_of(k))
+    sp, ss = _kv8_index(name, "start", start, shape[0])
+    cp, cs = _kv8_index(name, "counts", counts, shape[0])
+    with _C.on_device(dev):
+        (k, kst), (v, vst) = _kv8_rows(k), _kv8_rows(v)
+        _C.call("ml_kv8_append", c, k.data_ptr(), kst, v.data_ptr(), vst, shape[2], sp, ss, cp, cs,
+                _C.raw_stream(dev))
 
 
 def kv8_attention_cuda(q: Tensor, start: Tensor, counts: Tensor | None, k_codes: Tensor,
@@ -1071,26 +1076,23 @@ def kv8_attention_cuda(q: Tensor, start: Tensor, counts: Tensor | None, k_codes:
     """Attention of q [B, Hq, T, D] over the positions <= ``start`` + t of a
     cache held in 8 bits; returns [B, T, Hq, D] in q's dtype."""
     name = "kv8_attention"
-    _C.require_cuda(name, q, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)
+    dev = _same_device(name, q, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)
     c = _kv8_cache(name, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail, q.dtype)
-    if q.dim() != 4 or q.shape[0] != c.batch or q.shape[3] != c.head_dim or \
-            q.shape[1] == 0 or q.shape[1] % c.kv_heads:
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != c.batch or shape[3] != c.head_dim or shape[1] == 0 or \
+            shape[1] % c.kv_heads:
         raise RuntimeError(f"{name}: q {tuple(q.shape)} does not match the cache "
                            f"{tuple(k_codes.shape)}")
-    sp, ss = _kv8_index(name, "start", start, c.batch)
-    cp, cs = _kv8_index(name, "counts", counts, c.batch)
-    guard = _on_device(q)
-    if guard is not None:
-        with guard:
-            return kv8_attention_cuda(q, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail,
-                                      v_tail, scale)
-    B, Hq, T, D = q.shape
-    q, st = _kv8_rows(q)
-    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    nbytes = _C.load().ml_kv8_attention_workspace_bytes(ctypes.byref(c), Hq, T)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _C.call("ml_kv8_attention", ctypes.byref(c), q.data_ptr(), st, Hq, T, sp, ss, cp, cs,
-            float(scale), out.data_ptr(), _C.ptr(ws), nbytes, _C.stream_of(q))
+    B, Hq, T, D = shape
+    sp, ss = _kv8_index(name, "start", start, B)
+    cp, cs = _kv8_index(name, "counts", counts, B)
+    with _C.on_device(dev):
+        q, st = _kv8_rows(q)
+        out = q.new_empty((B, T, Hq, D))
+        nbytes = _C.load().ml_kv8_attention_workspace_bytes(c, Hq, T)
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _C.call("ml_kv8_attention", c, q.data_ptr(), st, Hq, T, sp, ss, cp, cs, scale,
+                out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _C.raw_stream(dev))
     return out
 
 
@@ -1110,28 +1112,26 @@ def sample_cuda(logits: Tensor, uniform: Tensor, temperature: Tensor | None,
                 min_p_value: float):
     """(id int64 [B], logprob fp32 [B]) of one token per row of logits [B, V]
     from uniform [B]; each parameter a [B] tensor or, without one, a value."""
-    _C.require_cuda("sample", logits, uniform, temperature, top_k, top_p, min_p)
+    dev = _same_device("sample", logits, uniform, temperature, top_k, top_p, min_p)
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise RuntimeError(f"sample: logits must be [B, V], not {tuple(logits.shape)}")
-    guard = _on_device(logits)
-    if guard is not None:
-        with guard:
-            return sample_cuda(logits, uniform, temperature, temperature_value, top_k,
-                               top_k_value, top_p, top_p_value, min_p, min_p_value)
     B, V = logits.shape
     code = _C.dtype_code(logits)
-    if logits.stride(1) != 1:
-        logits = logits.contiguous()
-    uniform, up = _sample_param("uniform", uniform, B, torch.float32)
-    temperature, tp = _sample_param("temperature", temperature, B, torch.float32)
-    top_k, kp = _sample_param("top_k", top_k, B, torch.int64)
-    top_p, pp = _sample_param("top_p", top_p, B, torch.float32)
-    min_p, mp = _sample_param("min_p", min_p, B, torch.float32)
-    index = torch.empty(B, dtype=torch.int64, device=logits.device)
-    logprob = torch.empty(B, dtype=torch.float32, device=logits.device)
-    _C.call("ml_sample", logits.data_ptr(), logits.stride(0), code, B, V, up, tp,
-            float(temperature_value), kp, int(top_k_value), pp, float(top_p_value), mp,
-            float(min_p_value), index.data_ptr(), logprob.data_ptr(), _C.stream_of(logits))
+    with _C.on_device(dev):
+        ld, one = logits.stride()
+        if one != 1 and V > 1:
+            logits = logits.contiguous()
+            ld = V
+        uniform, up = _sample_param("uniform", uniform, B, torch.float32)
+        temperature, tp = _sample_param("temperature", temperature, B, torch.float32)
+        top_k, kp = _sample_param("top_k", top_k, B, torch.int64)
+        top_p, pp = _sample_param("top_p", top_p, B, torch.float32)
+        min_p, mp = _sample_param("min_p", min_p, B, torch.float32)
+        index = logits.new_empty(B, dtype=torch.int64)
+        logprob = logits.new_empty(B, dtype=torch.float32)
+        _C.call("ml_sample", logits.data_ptr(), ld, code, B, V, up, tp, temperature_value, kp,
+                top_k_value, pp, top_p_value, mp, min_p_value, index.data_ptr(),
+                logprob.data_ptr(), _C.raw_stream(dev))
     return index, logprob
 
 

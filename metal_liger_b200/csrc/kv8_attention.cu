@@ -48,29 +48,36 @@ struct AttnArgs {
   const float* scale[2];    // [B, Hkv, L / block]
   Kv8Span span;
   int batch, kv_heads, group, rows, row_tiles, max_len, block;
+  int tiles_log2;           // tiles per block
   float qk_scale;           // scale * log2(e)
   void* out;                // [B, T, Hq, D]
   float* part;              // [2 * gridDim.x] pieces; null: a CTA per segment
   int ctas;                 // CTAs that share the flat list
+  bool split;               // the join: several CTAs to a segment
 };
 
-template <int D>
-struct Shape {
-  static constexpr int kWarps = D == 256 ? 4 : 8;
-  static constexpr int kTileBytes = 2 * kTile * D;  // K and V
-  static constexpr int MT = D / 16;                 // m-tiles of O^T
-};
+// A segment counts as this many tiles more than it has when the list is cut
+// into equal runs: reading its queries and writing its rows take a warp about
+// as long as one or two tiles.
+constexpr int kPad = 2;
 
-template <int D, int NT>
-struct Config : Shape<D> {
-  static constexpr int kStages = D == 64 ? 4 : NT == 1 ? 3 : 2;
-  static constexpr int kImage = NT * Shape<D>::MT * 4 * 32;  // floats of a piece
-  static constexpr int kStats = 3 * 8 * NT;
-  static constexpr int kPiece = kImage + kStats;             // floats, in the workspace
-  static constexpr size_t smem() {
-    return (size_t)Shape<D>::kWarps * (kStages * Shape<D>::kTileBytes + kImage * 4);
-  }
+// NW warps, each with a ring of units of 32 positions of K or of V.
+template <int D, int NT, int NW>
+struct Config {
+  static constexpr int kUnit = kTile * D;            // bytes
+  static constexpr int kUnits = D * NT >= 256 ? 24 * 1024 / kUnit : 12 * 1024 / kUnit;
+  static constexpr int MT = D / 16;                  // m-tiles of O^T
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kImage = NT * MT * 4 * 32;    // floats of a piece: acc ...
+  static constexpr int kStats = 3 * kRows;           // ... and m, l, mo of its rows
+  static constexpr int kPiece = kImage + kStats;     // in the workspace
+  static constexpr int kCtaPieces = 2 + NW;          // its first and last, its warps' first ones
+  static constexpr size_t smem() { return (size_t)NW * kUnits * kUnit; }
 };
+// Warps of a CTA of the list (two CTAs to an SM) ...
+constexpr int list_warps(int D, int NT) { return D * NT >= 256 ? 4 : 8; }
+// ... and of a CTA that has a segment to itself.
+constexpr int segment_warps(int D, int NT) { return 2 * list_warps(D, NT); }
 
 // ---------------------------------------------------------------------------
 // The flat list of tiles
@@ -88,57 +95,39 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) {
   const int n = c > 0 ? visible(a, b, c - 1) : 0;
   return n <= 0 ? 1 : (n + kTile - 1) / kTile;
 }
-__device__ __forceinline__ int64_t tiles_per_cta(int64_t total, int ctas, int warps) {
-  const int64_t even = (total + ctas - 1) / ctas;
+__device__ __forceinline__ int tiles_per_cta(int total, int ctas, int warps) {
+  const int even = (int)(((unsigned)total + ctas - 1) / (unsigned)ctas);
   return even > warps ? even : warps;
 }
 
-// Block-wide: the total number of tiles, and for each of `n` flat positions
-// the sequence that holds it and the tiles before that sequence.
-template <int THREADS>
-__device__ int64_t locate(const AttnArgs& a, int64_t* scan, int warps, int* at_b,
-                          int64_t* at_base, int64_t* per_cta) {
-  const int per = (a.batch + THREADS - 1) / THREADS;
-  const int64_t seg = (int64_t)a.kv_heads * a.row_tiles;
-  const int b0 = threadIdx.x * per;
-  int64_t mine = 0;
-  for (int b = b0; b < min(b0 + per, a.batch); ++b) mine += tiles_of(a, b) * seg;
-  // inclusive scan over the block
-  int64_t run = mine;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// One warp: the length of the list.
+__device__ __forceinline__ int total_tiles(const AttnArgs& a, int lane) {
+  const int per = a.kv_heads * a.row_tiles;
+  int total = 0;
+  for (int b = lane; b < a.batch; b += 32) total += (kPad + tiles_of(a, b)) * per;
+  return (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+}
+// One warp: the sequence that holds flat position `u` (below the total), and
+// what comes before it.
+__device__ __forceinline__ int find_sequence(const AttnArgs& a, int u, int lane, int* before) {
+  const int per = a.kv_heads * a.row_tiles;
+  int base = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int n = b0 + lane < a.batch ? (kPad + tiles_of(a, b0 + lane)) * per : 0;
+    int run = n;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += v;
-  }
-  if (lane == 31) scan[warp] = run;
-  __syncthreads();
-  int64_t total = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
-  }
-  int64_t lo = before + run - mine, hi = before + run;
-  const int64_t cta = tiles_per_cta(total, a.ctas, warps);
-  *per_cta = cta;
-  const int64_t sub = (cta + warps - 1) / warps;
-  for (int w = 0; w < warps; ++w) {
-    const int64_t u = blockIdx.x * cta + min(w * sub, cta);
-    if (u < lo || u >= hi) continue;
-    int64_t base = lo;
-    for (int b = b0;; ++b) {
-      const int64_t n = tiles_of(a, b) * seg;
-      if (u < base + n) {
-        at_b[w] = b;
-        at_base[w] = base;
-        break;
-      }
-      base += n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += v;
     }
+    const unsigned in = __ballot_sync(0xffffffffu, u < base + run);
+    if (in) {
+      const int f = __ffs(in) - 1;
+      *before = base + __shfl_sync(0xffffffffu, run - n, f);
+      return b0 + f;
+    }
+    base += __shfl_sync(0xffffffffu, run, 31);
   }
-  __syncthreads();
-  return total;
 }
 
 // ---------------------------------------------------------------------------
@@ -252,7 +241,7 @@ struct State {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], o);
   }
-  // As an image [register][lane] and stats [3][8 NT]
+  // As an image [register][lane], and m, l, mo by row
   __device__ __forceinline__ void save(float* image, float* stats, int lane) const {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -272,32 +261,6 @@ struct State {
         }
     }
   }
-  // Adds a saved piece (l summed over lanes in both).
-  __device__ __forceinline__ void join(const float* image, const float* stats, int lane) {
-    const int t = lane & 3;
-    float ka[NT][2], kb[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = n * 8 + 2 * t + c;
-        const float pm = stats[r], pl = stats[8 * NT + r], po = stats[16 * NT + r];
-        const float nm = fmaxf(m[n][c], pm), no = fmaxf(mo[n][c], po);
-        l[n][c] = l[n][c] * rel2(m[n][c], nm) + pl * rel2(pm, nm);
-        ka[n][c] = rel2(mo[n][c], no);
-        kb[n][c] = rel2(po, no);
-        m[n][c] = nm;
-        mo[n][c] = no;
-      }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          acc[n][j][e] = acc[n][j][e] * ka[n][e & 1] +
-                         image[((n * (D / 16) + j) * 4 + e) * 32 + lane] * kb[n][e & 1];
-  }
   template <typename T>
   __device__ __forceinline__ void write(const AttnArgs& a, int b, int kvh, int rt, int lane) const {
     const int g = lane >> 2, t = lane & 3;
@@ -308,8 +271,8 @@ struct State {
         const int r = (rt * NT + n) * 8 + 2 * t + c;
         if (r >= a.rows) continue;
         const int tok = r / a.group, h = kvh * a.group + r % a.group;
-        const float f = visible(a, b, tok) > 0 ? rel2(mo[n][c], m[n][c]) / l[n][c] : 0.f;
-        const bool none = f == 0.f;  // no position, or all V blocks zero
+        const bool none = visible(a, b, tok) == 0;
+        const float f = rel2(mo[n][c], m[n][c]) / l[n][c];
         T* dst = static_cast<T*>(a.out) +
                  (((int64_t)b * a.span.tokens + tok) * (a.kv_heads * a.group) + h) * D;
         constexpr int PER = D == 64 ? 8 : 16;  // consecutive dims of a lane
@@ -341,28 +304,44 @@ struct Query {
   int lim[NT][2];
   int lim_min, lim_max;  // over the rows that see anything
 
+  // The rows as they are, into `frag` ...
   template <typename T>
-  __device__ __forceinline__ void load(const AttnArgs& a, int b, int kvh, int rt, int lane) {
+  __device__ __forceinline__ void fetch(const AttnArgs& a, int b, int seg, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    lim_min = a.max_len;
-    lim_max = 0;
+    const int kvh = seg / a.row_tiles, rt = seg % a.row_tiles;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = (rt * NT + n) * 8 + g;
       const int tok = r / a.group, h = kvh * a.group + r % a.group;
       const T* src = static_cast<const T*>(a.q) + b * a.sq[0] + h * a.sq[1] + tok * a.sq[2];
-      uint4 raw[D / 32];
-      uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < D / 64; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          uint4& x = raw[2 * i + u];
-          x = r < a.rows ? *reinterpret_cast<const uint4*>(src + i * 64 + t * 16 + u * 8)
-                         : make_uint4(0, 0, 0, 0);
-          top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                       __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+          const uint4 x = r < a.rows
+                              ? *reinterpret_cast<const uint4*>(src + i * 64 + t * 16 + u * 8)
+                              : make_uint4(0, 0, 0, 0);
+          // words of 2 dims: k-steps 4 i + 2 u and the next, two registers each
+          frag[n][4 * i + 2 * u][0] = x.x;
+          frag[n][4 * i + 2 * u][1] = x.y;
+          frag[n][4 * i + 2 * u + 1][0] = x.z;
+          frag[n][4 * i + 2 * u + 1][1] = x.w;
         }
+    }
+  }
+  // ... and scaled to fp16.
+  template <typename T>
+  __device__ __forceinline__ void finish(const AttnArgs& a, int b, int seg, int lane) {
+    const int t = lane & 3;
+    const int rt = seg % a.row_tiles;
+    lim_min = a.max_len;
+    lim_max = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        top = __vmaxu2(top, __vmaxu2(frag[n][i][0] & 0x7fff7fffu, frag[n][i][1] & 0x7fff7fffu));
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -370,24 +349,22 @@ struct Query {
       const uint16_t tb = (uint16_t)top;
       memcpy(&tv, &tb, 2);
       const float amax = to_f32(tv);
-      // 2^-e with 2^e the largest power of two <= amax; 1 for zero, inf, NaN
-      // rows and below 2^-100 (whose scores are nothing anyway)
+      // 2^-e with 2^e the largest power of two <= amax; 1 for zero, inf and NaN
+      // rows, and below 2^-100, where the scores are nothing anyway
       const uint32_t e = __float_as_uint(amax) & 0x7f800000u;
-      const bool ok = e > 0x0d800000u && e < 0x7f000000u;
-      const float down = ok ? __uint_as_float(0x7f000000u - e) : e >= 0x7f000000u && amax <= 3.4028235e38f ? 0x1p-127f : 1.f;
-      const float up = ok ? __uint_as_float(e) : e >= 0x7f000000u && amax <= 3.4028235e38f ? 0x1p127f : 1.f;
+      const bool finite = amax <= 3.4028235e38f;
+      const float down = !finite || e <= 0x0d800000u ? 1.f
+                         : e < 0x7f000000u           ? __uint_as_float(0x7f000000u - e)
+                                                     : 0x1p-127f;
+      const float up = !finite || e <= 0x0d800000u ? 1.f : __uint_as_float(e);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 2; ++k) {
           T two[2];
-          memcpy(two, &w[k], 4);
-          // words of 2 dims: k-step 4 (i / 2) + 2 (i % 2) + k / 2, register k & 1
-          frag[n][(i / 2) * 4 + (i % 2) * 2 + k / 2][k & 1] =
-              half2_bits(to_f32(two[0]) * down, to_f32(two[1]) * down);
+          memcpy(two, &frag[n][i][k], 4);
+          frag[n][i][k] = half2_bits(to_f32(two[0]) * down, to_f32(two[1]) * down);
         }
-      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         mul[n][c] = __shfl_sync(0xffffffffu, up, (2 * t + c) * 4) * a.qk_scale;
@@ -404,11 +381,12 @@ struct Query {
   }
 };
 
-// One tile of 32 positions, the first of them `pos`.
+// Scores and probabilities of one tile of 32 positions, the first of them
+// `pos`, as B fragments of the second product.
 template <int D, int NT, int FMT, bool MASK>
-__device__ __forceinline__ void tile_step(State<D, NT>& st, const Query<D, NT>& q,
-                                          const uint8_t* ks, const uint8_t* vs, float k_scale,
-                                          float v_scale, int pos, int lane) {
+__device__ __forceinline__ void score_step(State<D, NT>& st, const Query<D, NT>& q,
+                                           const uint8_t* ks, float k_scale, float v_scale,
+                                           uint32_t (&p)[2][NT][2], int pos, int lane) {
   const int g = lane >> 2, t = lane & 3;
   float s[2][NT][4];
 #pragma unroll
@@ -440,8 +418,7 @@ __device__ __forceinline__ void tile_step(State<D, NT>& st, const Query<D, NT>& 
         for (int n = 0; n < NT; ++n) mma(s[i][n], f, q.frag[n][h * 4 + w]);
       }
   }
-  const float lv = log2f(v_scale);
-  uint32_t p[2][NT][2];
+  const float lv = __log2f(v_scale);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float top[2];
@@ -498,7 +475,15 @@ __device__ __forceinline__ void tile_step(State<D, NT>& st, const Query<D, NT>& 
       for (int u = 0; u < 2; ++u)
         p[i][n][u] = transpose8(half2_bits(s[i][n][2 * u], s[i][n][2 * u + 1]));
   }
-  // dims: a lane's 16 (8 of 64) consecutive ones of each 128
+}
+
+// Adds the tile's V rows, weighted.  A lane holds 16 (8 of 64) consecutive dims
+// of each 128.
+template <int D, int NT, int FMT, bool MASK>
+__device__ __forceinline__ void value_step(State<D, NT>& st, const Query<D, NT>& q,
+                                           const uint8_t* vs, const uint32_t (&p)[2][NT][2],
+                                           int pos, int lane) {
+  const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int h = 0; h < (D + 127) / 128; ++h)
 #pragma unroll
@@ -545,42 +530,73 @@ __device__ __forceinline__ void tile_step(State<D, NT>& st, const Query<D, NT>& 
     }
 }
 
-// Position in the flat list: tile `tile` of `tiles` of segment `seg` (kv head x
-// row tile) of sequence b.
+// Position `u` in the flat list: tile `tile` of `tiles` of segment `seg` (kv
+// head x row tile) of sequence b.
 struct Cursor {
-  int b, seg, tile, tiles;
+  int u, b, seg, tile, tiles;
 
-  __device__ __forceinline__ void set(const AttnArgs& a, int b_, int64_t offset) {
+  // The first tile at or after u, which lies `offset` into sequence b_.
+  __device__ __forceinline__ void set(const AttnArgs& a, int b_, int offset) {
     b = b_;
     tiles = tiles_of(a, b);
-    seg = (int)(offset / tiles);
-    tile = (int)(offset - (int64_t)seg * tiles);
+    const unsigned per = tiles + kPad;
+    seg = (int)((unsigned)offset / per);
+    const int x = offset - seg * (int)per;
+    u += x < kPad ? kPad - x : 0;
+    tile = x < kPad ? 0 : x - kPad;
   }
-  __device__ __forceinline__ void next(const AttnArgs& a) {
-    if (++tile < tiles) return;
+  // true where another segment begins
+  __device__ __forceinline__ bool next(const AttnArgs& a) {
+    ++u;
+    if (++tile < tiles) return false;
+    u += kPad;
     tile = 0;
-    if (++seg < a.kv_heads * a.row_tiles) return;
-    seg = 0;
-    if (++b < a.batch) tiles = tiles_of(a, b);
+    if (++seg == a.kv_heads * a.row_tiles) {
+      seg = 0;
+      if (++b < a.batch) tiles = tiles_of(a, b);
+    }
+    return true;
   }
 };
 
+// A cursor with this lane's place in the cache.
 template <int D>
-__device__ __forceinline__ void load_tile(const AttnArgs& a, const Cursor& c, uint32_t dst,
-                                          uint32_t scales, int lane) {
-  const int64_t bh = (int64_t)c.b * a.kv_heads + c.seg / a.row_tiles;
-  const int64_t off = (bh * a.max_len + (int64_t)c.tile * kTile) * D;
-  constexpr int CPR = D / 16;
-#pragma unroll
-  for (int i = 0; i < kTile * CPR / 32; ++i) {
-    const int x = i * 32 + lane;
-    const int r = x / CPR, ch = x % CPR;
-    cp_async16(dst + r * D + k_chunk<D>(r, ch) * 16, a.codes[0] + off + x * 16);
-    cp_async16(dst + kTile * D + r * D + v_chunk<D>(r, ch) * 16, a.codes[1] + off + x * 16);
+struct Loader {
+  Cursor c;
+  int64_t off;  // of its 16 bytes of the tile's first rows
+  int scale;    // index of the segment's first block
+
+  __device__ __forceinline__ void point(const AttnArgs& a, int lane) {
+    const int bh = c.b * a.kv_heads + c.seg / a.row_tiles;
+    off = ((int64_t)bh * a.max_len + (int64_t)c.tile * kTile) * D + lane * 16;
+    scale = bh * (a.max_len / a.block);
   }
-  if (lane < 2)
+  __device__ __forceinline__ void next(const AttnArgs& a, int lane) {
+    if (c.next(a)) {
+      if (c.b < a.batch) point(a, lane);
+    } else {
+      off += kTile * D;
+    }
+  }
+};
+
+// The K unit of a tile brings the tile's two scales along.
+template <int D, int WHICH>
+__device__ __forceinline__ void load_unit(const AttnArgs& a, const Loader<D>& from, uint32_t dst,
+                                          uint32_t scales, int lane) {
+  constexpr int CPR = D / 16;
+  constexpr int RPP = 32 / CPR;  // rows per pass of the warp
+  const int r0 = lane / CPR, ch = lane % CPR;
+  const uint8_t* src = a.codes[WHICH] + from.off;
+#pragma unroll
+  for (int i = 0; i < kTile / RPP; ++i) {
+    const int r = r0 + i * RPP;
+    const int at = WHICH == 0 ? k_chunk<D>(r, ch) : v_chunk<D>(r, ch);
+    cp_async16(dst + r * D + at * 16, src + i * 512);
+  }
+  if (WHICH == 0 && lane < 2)
     cp_async4(scales + lane * 4,
-              a.scale[lane] + bh * (a.max_len / a.block) + (int64_t)c.tile * kTile / a.block);
+              (lane ? a.scale[1] : a.scale[0]) + from.scale + (from.c.tile >> a.tiles_log2));
 }
 
 // A piece of a segment that its warp did not see whole.
@@ -588,196 +604,364 @@ struct Piece {
   int b, seg, lo, hi, tiles;  // tiles [lo, hi) of `tiles`; hi = 0: none
 };
 
-template <typename T, int FMT, int D, int NT>
-__global__ void __launch_bounds__(32 * Shape<D>::kWarps, 1)
+// Four values of a joined image, of one lane and m-tile: to the output ...
+template <typename T, int D, int NT>
+__device__ __forceinline__ void write_item(const AttnArgs& a, int b, int seg, int item,
+                                           const float* o) {
+  using C = Config<D, NT, 8>;
+  const int l = item & 31, j = (item >> 5) % C::MT, n = (item >> 5) / C::MT;
+  const int t = l & 3, g = l >> 2;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int r = (seg % a.row_tiles) * C::kRows + n * 8 + 2 * t + c;
+    if (r >= a.rows) continue;
+    const int tok = r / a.group, h = (seg / a.row_tiles) * a.group + r % a.group;
+    constexpr int PER = D == 64 ? 8 : 16;  // consecutive dims of a lane
+    T* dst = static_cast<T*>(a.out) +
+             (((int64_t)b * a.span.tokens + tok) * (a.kv_heads * a.group) + h) * D +
+             (j * 2 / PER) * 128 + g * PER + j * 2 % PER;
+    T two[2] = {from_f32<T>(o[c]), from_f32<T>(o[2 + c])};
+    uint32_t w;
+    memcpy(&w, two, 4);
+    *reinterpret_cast<uint32_t*>(dst) = w;
+  }
+}
+// ... from the images of every STEP-th piece of [from, to), each times its
+// row's factor (negative: the row sees nothing, its images hold anything).
+template <int D, int NT, int STEP, typename Image>
+__device__ __forceinline__ void sum_item(int item, int from, int to, const Image& image,
+                                         const float (*factor)[8 * NT], float* o) {
+  using C = Config<D, NT, 8>;
+  const int l = item & 31, n = (item >> 5) / C::MT, r = n * 8 + 2 * (l & 3);
+  o[0] = o[1] = o[2] = o[3] = 0.f;
+#pragma unroll 4
+  for (int i = from; i < to; i += STEP) {
+    const float* src = image(i) + (item >> 5) * 128 + l;
+    const float2 k = *reinterpret_cast<const float2*>(&factor[i][r]);
+    const float x[4] = {src[0], src[32], src[64], src[96]};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float f = e & 1 ? k.y : k.x;
+      o[e] += f < 0.f ? 0.f : x[e] * f;  // a zero factor still passes NaN on
+    }
+  }
+}
+
+// A segment with pieces in this CTA: entries [from, to) of the list of pieces.
+struct Run {
+  int from, to, b, seg;
+  bool whole;  // all of it is here
+  bool begun;  // it began in an earlier CTA
+};
+
+template <typename T, int FMT, int D, int NT, int NW>
+__global__ void __launch_bounds__(32 * NW, NW == list_warps(D, NT) ? 2 : 1)
 kv8_attention_kernel(const __grid_constant__ AttnArgs a) {
-  using C = Config<D, NT>;
-  constexpr int NW = C::kWarps;
+  using C = Config<D, NT, NW>;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int64_t scan[NW], at_base[NW];
-  __shared__ int at_b[NW];
   __shared__ Piece pieces[2 * NW];
   __shared__ float stats[2 * NW][C::kStats];
-  __shared__ float scales[NW][C::kStages][2];
+  __shared__ __align__(8) float factor[2 * NW][C::kRows];
+  __shared__ Run runs[2 * NW];
+  __shared__ int entry[2 * NW];  // of the list, by rank: 2 * warp + slot
+  __shared__ float scales[NW][C::kUnits][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint8_t* ring = smem + (size_t)warp * C::kStages * C::kTileBytes;
-  float* first_image = reinterpret_cast<float*>(smem + (size_t)NW * C::kStages * C::kTileBytes) +
-                       (size_t)warp * C::kImage;
+  uint8_t* ring = smem + (size_t)warp * C::kUnits * C::kUnit;
+  float* scratch = a.part + (int64_t)blockIdx.x * C::kCtaPieces * C::kPiece;
 
   pdl_wait();
   pdl_release();
-  // this warp's run [lo, hi) of the list, and where it starts
-  int64_t lo, hi, cta_lo = 0;
+  // this warp's run of the list: from `cur` up to `hi`
+  int hi;
   Cursor cur;
   if (a.part == nullptr) {  // a CTA per segment
-    const int seg = a.kv_heads * a.row_tiles;
-    const int b = blockIdx.x / seg, s = blockIdx.x % seg;
-    const int n = tiles_of(a, b), sub = (n + NW - 1) / NW;
-    lo = min(warp * sub, n);
-    hi = min(lo + sub, (int64_t)n);
-    cur.b = b;
-    cur.seg = s;
-    cur.tiles = n;
-    cur.tile = (int)lo;
+    const int segs = a.kv_heads * a.row_tiles;
+    cur.b = blockIdx.x / segs;
+    cur.seg = blockIdx.x % segs;
+    cur.tiles = tiles_of(a, cur.b);
+    const int sub = (cur.tiles + NW - 1) / NW;
+    cur.u = cur.tile = min(warp * sub, cur.tiles);
+    hi = min(cur.u + sub, cur.tiles);
   } else {
-    int64_t per_cta;
-    const int64_t total = locate<32 * NW>(a, scan, NW, at_b, at_base, &per_cta);
-    cta_lo = blockIdx.x * per_cta;
-    const int64_t cta_hi = min(total, cta_lo + per_cta), sub = (per_cta + NW - 1) / NW;
-    lo = min(cta_lo + warp * sub, cta_hi);
-    hi = min(lo + sub, cta_hi);
-    if (lo < hi) cur.set(a, at_b[warp], lo - at_base[warp]);
+    const int total = total_tiles(a, lane);
+    const int per_cta = tiles_per_cta(total, a.ctas, NW), sub = (per_cta + NW - 1) / NW;
+    const int cta_lo = (int)min((int64_t)blockIdx.x * per_cta, (int64_t)total);
+    const int cta_hi = min(total - cta_lo, per_cta) + cta_lo;
+    cur.u = min(cta_lo + warp * sub, cta_hi);
+    hi = min(cur.u + sub, cta_hi);
+    if (cur.u < hi) {
+      int before;
+      const int b = find_sequence(a, cur.u, lane, &before);
+      cur.set(a, b, cur.u - before);
+    }
   }
 
   if (lane < 2) pieces[2 * warp + lane].hi = 0;
   __syncwarp();
-  if (lo < hi) {
+  if (cur.u < hi) {
     const uint32_t ring_u = smem_u32_of(ring), scales_u = smem_u32_of(&scales[warp][0][0]);
-    Cursor ahead = cur;
-    const int64_t n = hi - lo;
-#pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) {
-      if (i < n) {
-        load_tile<D>(a, ahead, ring_u + i * C::kTileBytes, scales_u + i * 8, lane);
-        ahead.next(a);
-      }
-      cp_commit();
-    }
     State<D, NT> st;
     Query<D, NT> q;
-    int stage = 0, piece_lo = 0;
-    bool fresh = true;
-    for (int64_t i = 0; i < n; ++i) {
-      if (fresh) {
-        q.template load<T>(a, cur.b, cur.seg / a.row_tiles, cur.seg % a.row_tiles, lane);
-        st.clear();
-        piece_lo = cur.tile;
-        fresh = false;
-      }
-      cp_wait<C::kStages - 2>();
-      __syncwarp();
-      if (i + C::kStages - 1 < n) {
-        const int to = stage == 0 ? C::kStages - 1 : stage - 1;
-        load_tile<D>(a, ahead, ring_u + to * C::kTileBytes, scales_u + to * 8, lane);
-        ahead.next(a);
+    // the queries first: behind the first units they would wait for those
+    q.template fetch<T>(a, cur.b, cur.seg, lane);
+    Loader<D> ahead;
+    ahead.c = cur;
+    ahead.point(a, lane);
+    // units are K and V of the tiles in turn
+    int to = 0;
+    bool odd = false;
+    auto load_next = [&] {
+      if (ahead.c.u < hi) {
+        if (odd) {
+          load_unit<D, 1>(a, ahead, ring_u + to * C::kUnit, 0, lane);
+          ahead.next(a, lane);
+        } else {
+          load_unit<D, 0>(a, ahead, ring_u + to * C::kUnit, scales_u + to * 8, lane);
+        }
+        odd = !odd;
+        to = to == C::kUnits - 1 ? 0 : to + 1;
       }
       cp_commit();
-      const uint8_t* ks = ring + stage * C::kTileBytes;
+    };
+#pragma unroll 1
+    for (int i = 0; i < C::kUnits - 1; ++i) load_next();
+    int at = 0, piece_lo = cur.tile;
+    q.template finish<T>(a, cur.b, cur.seg, lane);
+    st.clear();
+#pragma unroll 1
+    while (true) {
       const int pos = cur.tile * kTile;
-      const float k_scale = scales[warp][stage][0], v_scale = scales[warp][stage][1];
-      if (pos + kTile <= q.lim_min)
-        tile_step<D, NT, FMT, false>(st, q, ks, ks + kTile * D, k_scale, v_scale, pos, lane);
+      const bool open = pos + kTile <= q.lim_min;
+      uint32_t p[2][NT][2];
+      cp_wait<C::kUnits - 2>();
+      __syncwarp();
+      load_next();  // into the unit read last, which every lane is done with
+      const float k_scale = scales[warp][at][0], v_scale = scales[warp][at][1];
+      if (open)
+        score_step<D, NT, FMT, false>(st, q, ring + at * C::kUnit, k_scale, v_scale, p, pos, lane);
       else
-        tile_step<D, NT, FMT, true>(st, q, ks, ks + kTile * D, k_scale, v_scale, pos, lane);
-      stage = stage == C::kStages - 1 ? 0 : stage + 1;
-      const bool ends = cur.tile + 1 == cur.tiles;
-      if (ends || i + 1 == n) {
-        st.sum_l();
-        if (ends && piece_lo == 0) {
-          st.template write<T>(a, cur.b, cur.seg / a.row_tiles, cur.seg % a.row_tiles, lane);
-        } else {
-          // the run's first piece has a place of its own, its last one takes
-          // the ring, which nothing uses any more
-          const int slot = i + 1 - (cur.tile + 1 - piece_lo) == 0 ? 0 : 1;
-          if (slot == 1) {
-            cp_wait<0>();
-            __syncwarp();
-          }
-          st.save(slot == 0 ? first_image : reinterpret_cast<float*>(ring), stats[2 * warp + slot],
-                  lane);
-          if (lane == 0)
-            pieces[2 * warp + slot] = {cur.b, cur.seg, piece_lo, cur.tile + 1, cur.tiles};
+        score_step<D, NT, FMT, true>(st, q, ring + at * C::kUnit, k_scale, v_scale, p, pos, lane);
+      at = at == C::kUnits - 1 ? 0 : at + 1;
+      cp_wait<C::kUnits - 2>();
+      __syncwarp();
+      load_next();
+      if (open)
+        value_step<D, NT, FMT, false>(st, q, ring + at * C::kUnit, p, pos, lane);
+      else
+        value_step<D, NT, FMT, true>(st, q, ring + at * C::kUnit, p, pos, lane);
+      at = at == C::kUnits - 1 ? 0 : at + 1;
+
+      const Cursor was = cur;
+      const bool ends = cur.next(a), last = cur.u >= hi;
+      if (!ends && !last) continue;
+      st.sum_l();
+      if (ends && piece_lo == 0) {
+        st.template write<T>(a, was.b, was.seg / a.row_tiles, was.seg % a.row_tiles, lane);
+      } else {
+        // the run's last piece takes the ring, which nothing uses any more; a
+        // first one before other segments goes to the workspace
+        const int slot = last ? 1 : 0;
+        if (last) {
+          cp_wait<0>();
+          __syncwarp();
         }
-        fresh = true;
+        st.save(last ? reinterpret_cast<float*>(ring) : scratch + (2 + warp) * C::kPiece,
+                stats[2 * warp + slot], lane);
+        if (lane == 0)
+          pieces[2 * warp + slot] = {was.b, was.seg, piece_lo, was.tile + 1, was.tiles};
       }
-      cur.next(a);
+      if (last) break;
+      q.template fetch<T>(a, cur.b, cur.seg, lane);
+      q.template finish<T>(a, cur.b, cur.seg, lane);
+      st.clear();
+      piece_lo = cur.tile;
     }
   }
   cp_wait<0>();
   __syncthreads();
-  // Join the pieces of a segment: runs of consecutive entries, a warp per run.
-  int run = 0;
-  for (int e = 0; e < 2 * NW;) {
-    const Piece p = pieces[e];
-    if (p.hi == 0) {
-      ++e;
-      continue;
-    }
-    int last = e, f = e + 1;
-    for (; f < 2 * NW; ++f) {
-      const Piece& o = pieces[f];
-      if (o.hi == 0) continue;
-      if (o.b != p.b || o.seg != p.seg) break;
-      last = f;
-    }
-    if (run++ % NW == warp) {
-      State<D, NT> st;
-      st.clear();
-      for (int x = e; x <= last; ++x) {
-        if (pieces[x].hi == 0) continue;
-        const float* image =
-            x & 1 ? reinterpret_cast<const float*>(smem + (size_t)(x >> 1) * C::kStages * C::kTileBytes)
-                  : reinterpret_cast<const float*>(smem + (size_t)NW * C::kStages * C::kTileBytes) +
-                        (size_t)(x >> 1) * C::kImage;
-        st.join(image, stats[x], lane);
+
+  // Join the pieces: those of one segment follow one another.  A lane per
+  // entry finds the runs; then a warp per row makes the entries' factors with
+  // reductions inside the runs.
+  static_assert(2 * NW <= 32, "an entry per lane");
+  Piece mine = {0, 0, 0, 0, 0};
+  if (lane < 2 * NW) mine = pieces[lane];
+  const unsigned valid = __ballot_sync(0xffffffffu, mine.hi > 0);
+  if (valid == 0) return;
+  const unsigned below = (1u << lane) - 1, upto = below | (1u << lane);
+  const int prev = (valid & below) ? 31 - __clz(valid & below) : lane;
+  const int prev_b = __shfl_sync(0xffffffffu, mine.b, prev);
+  const int prev_seg = __shfl_sync(0xffffffffu, mine.seg, prev);
+  const bool starts = mine.hi > 0 && ((valid & below) == 0 || prev_b != mine.b || prev_seg != mine.seg);
+  const unsigned head = __ballot_sync(0xffffffffu, starts);
+  const int my_head = (head & upto) ? 31 - __clz(head & upto) : lane;
+  const int end = (head & ~upto) ? __ffs(head & ~upto) - 1 : 32;  // of this lane's run
+  const unsigned in_run = valid & (end == 32 ? 0xffffffffu : (1u << end) - 1);
+  const int head_lo = __shfl_sync(0xffffffffu, mine.lo, my_head);
+  const int last_hi = __shfl_sync(0xffffffffu, mine.hi, in_run ? 31 - __clz(in_run) : 0);
+  const bool whole = head_lo == 0 && last_hi == mine.tiles;
+  const int rank = __popc(valid & below);
+  if (warp == 0 && mine.hi > 0) {
+    entry[rank] = lane;
+    if (starts)
+      runs[__popc(head & below)] = {rank, __popc(in_run), mine.b, mine.seg, whole, mine.lo > 0};
+  }
+  for (int r = warp; r < C::kRows; r += NW) {
+    const bool on = mine.hi > 0;
+    const float m = on ? stats[lane][r] : -INFINITY;
+    const float l = on ? stats[lane][C::kRows + r] : 0.f;
+    const float mo = on ? stats[lane][2 * C::kRows + r] : -INFINITY;
+    float M = m, MO = mo;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float x = __shfl_down_sync(0xffffffffu, M, o), y = __shfl_down_sync(0xffffffffu, MO, o);
+      if (lane + o < end) {
+        M = fmaxf(M, x);
+        MO = fmaxf(MO, y);
       }
-      if (p.lo == 0 && pieces[last].hi == p.tiles) {
-        st.template write<T>(a, p.b, p.seg / a.row_tiles, p.seg % a.row_tiles, lane);
-      } else {
-        // slot 0: the piece the CTA's run starts with
-        const bool starts = e == 0;
-        float* to = a.part + (int64_t)(2 * blockIdx.x + (starts ? 0 : 1)) * C::kPiece;
-        st.save(to, to + C::kImage, lane);
+    }
+    M = __shfl_sync(0xffffffffu, M, my_head);
+    MO = __shfl_sync(0xffffffffu, MO, my_head);
+    float L = on ? l * rel2(m, M) : 0.f;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float x = __shfl_down_sync(0xffffffffu, L, o);
+      if (lane + o < end) L += x;
+    }
+    L = __shfl_sync(0xffffffffu, L, my_head);
+    if (on) {
+      const int row = (mine.seg % a.row_tiles) * C::kRows + r;
+      const bool sees = row < a.rows && visible(a, mine.b, row / a.group) > 0;
+      factor[rank][r] = sees ? rel2(mo, MO) * (whole ? rel2(MO, M) / L : 1.f) : -1.f;
+      if (starts && !whole) {
+        // place 0 for a segment that began in an earlier CTA, 1 for one that
+        // goes on in the next
+        float* to = scratch + (mine.lo > 0 ? 0 : 1) * C::kPiece + C::kImage;
+        to[r] = M;
+        to[C::kRows + r] = L;
+        to[2 * C::kRows + r] = MO;
       }
     }
-    e = f;
+  }
+  __syncthreads();
+  auto image = [&](int i) {
+    const int e = entry[i];
+    return e & 1 ? reinterpret_cast<const float*>(smem + (size_t)(e >> 1) * C::kUnits * C::kUnit)
+                 : static_cast<const float*>(scratch + (2 + (e >> 1)) * C::kPiece);
+  };
+  constexpr int kItems = C::kImage / 4;
+  for (int x = threadIdx.x; x < __popc(head) * kItems; x += 32 * NW) {
+    const Run& run = runs[x / kItems];
+    const int item = x % kItems;
+    float o[4];
+    sum_item<D, NT, 1>(item, run.from, run.to, image, factor, o);
+    if (run.whole) {
+      write_item<T, D, NT>(a, run.b, run.seg, item, o);
+    } else {
+      float* to = scratch + (run.begun ? 0 : 1) * C::kPiece + (item >> 5) * 128 + (item & 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e * 32] = o[e];
+    }
   }
 }
 
-// Joins the segments that cross CTAs, a warp each.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) kv8_attention_join(const __grid_constant__ AttnArgs a) {
-  using C = Config<D, NT>;
-  __shared__ int64_t red[8];
-  pdl_wait();
-  pdl_release();
+// Joins the segments that cross CTAs.  The pieces' statistics become one factor
+// per piece and row (a row per warp, lanes over the pieces).  Few segments have
+// many pieces: a CTA takes 32 items of one, a warp every kJoinGroups-th piece,
+// so that few loads follow one another, and the warps' sums are added in
+// order.  Many segments have few: a CTA takes one, a warp 32 items of all its
+// pieces.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinGroups = kJoinThreads / 32;
+constexpr int kMaxCtas = 640;  // of the list
+
+template <typename T, int D, int NT, int NW>
+__global__ void __launch_bounds__(kJoinThreads)
+kv8_attention_join(const __grid_constant__ AttnArgs a) {
+  using C = Config<D, NT, NW>;
+  constexpr int kParts = C::kImage / 4 / 32;  // of 32 items
+  __shared__ __align__(8) float factor[kMaxCtas][C::kRows];
+  __shared__ float4 sums[kJoinGroups][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per_b = a.kv_heads * a.row_tiles;
-  // the CTA's segments are of one sequence: tiles before it, and in all
-  const int chunks = (per_b + 3) / 4;
-  const int b = blockIdx.x / chunks;
-  int64_t before = 0, total = 0;
-  for (int i = threadIdx.x; i < a.batch; i += 128) {
-    const int64_t n = (int64_t)tiles_of(a, i) * per_b;
+  const int segment = a.split ? blockIdx.x / kParts : blockIdx.x;
+  const int b = segment / per_b, seg = segment % per_b;
+  // start and counts may be read before the wait: this grid starts when the
+  // first kernel's CTAs have passed theirs, and that kernel writes neither
+  int before = 0, total = 0;  // of the list, before the segment's sequence and in all
+  for (int i = lane; i < a.batch; i += 32) {
+    const int n = (kPad + tiles_of(a, i)) * per_b;
     total += n;
     if (i < b) before += n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  if (lane == 0) {
-    red[warp] = before;
-    red[4 + warp] = total;
+  before = (int)__reduce_add_sync(0xffffffffu, (unsigned)before);
+  total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+  const int per_cta = tiles_per_cta(total, a.ctas, NW);
+  const int n = tiles_of(a, b);
+  const int lo = before + seg * (n + kPad) + kPad;  // its first tile
+  const int c0 = lo / per_cta;
+  const int count = (lo + n - 1) / per_cta - c0 + 1;
+  const int rt = seg % a.row_tiles;
+  pdl_wait();
+  pdl_release();
+  if (count == 1) return;  // whole in one CTA, which wrote it
+  auto piece = [&](int i) -> const float* {
+    return a.part + ((int64_t)(c0 + i) * C::kCtaPieces + (i == 0 ? 1 : 0)) * C::kPiece;
+  };
+  for (int r = warp; r < C::kRows; r += kJoinThreads / 32) {
+    const bool sees = rt * C::kRows + r < a.rows && visible(a, b, (rt * C::kRows + r) / a.group) > 0;
+    float M = -INFINITY, MO = -INFINITY, L = 0.f;
+    float m = -INFINITY, l = 0.f, mo = -INFINITY;  // of this lane's first piece
+    if (lane < count) {
+      const float* st = piece(lane) + C::kImage + r;
+      m = st[0];
+      l = st[C::kRows];
+      mo = st[2 * C::kRows];
+    }
+    M = m;
+    MO = mo;
+    for (int i = lane + 32; i < count; i += 32) {
+      const float* st = piece(i) + C::kImage + r;
+      M = fmaxf(M, st[0]);
+      MO = fmaxf(MO, st[2 * C::kRows]);
+    }
+    M = warp_max(M);
+    MO = warp_max(MO);
+    L = l * rel2(m, M);
+    for (int i = lane + 32; i < count; i += 32) {
+      const float* st = piece(i) + C::kImage + r;
+      L += st[C::kRows] * rel2(st[0], M);
+    }
+    L = warp_sum(L);
+    const float f = rel2(MO, M) / L;
+    for (int i = lane; i < count; i += 32) {
+      const float x = i == lane ? mo : piece(i)[C::kImage + 2 * C::kRows + r];
+      factor[i][r] = sees ? rel2(x, MO) * f : -1.f;
+    }
   }
   __syncthreads();
-  before = red[0] + red[1] + red[2] + red[3];
-  total = red[4] + red[5] + red[6] + red[7];
-  const int seg = (blockIdx.x % chunks) * 4 + warp;
-  if (seg >= per_b) return;
-  const int64_t per_cta = tiles_per_cta(total, a.ctas, C::kWarps);
-  const int n = tiles_of(a, b);
-  const int64_t lo = before + (int64_t)seg * n, hi = lo + n;
-  const int64_t c0 = lo / per_cta, c1 = (hi - 1) / per_cta;
-  if (c0 == c1) return;
-  State<D, NT> st;
-  st.clear();
-  for (int64_t c = c0; c <= c1; ++c) {
-    const float* p = a.part + (2 * c + (c == c0 && lo > c * per_cta ? 1 : 0)) * C::kPiece;
-    st.join(p, p + C::kImage, lane);
+  float o[4];
+  if (!a.split) {
+    for (int x = threadIdx.x; x < kParts * 32; x += kJoinThreads) {
+      sum_item<D, NT, 1>(x, 0, count, piece, factor, o);
+      write_item<T, D, NT>(a, b, seg, x, o);
+    }
+    return;
   }
-  st.template write<T>(a, b, seg / a.row_tiles, seg % a.row_tiles, lane);
+  const int item = blockIdx.x % kParts * 32 + lane;
+  sum_item<D, NT, kJoinGroups>(item, warp, count, piece, factor, o);
+  sums[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
+  __syncthreads();
+  if (warp > 0) return;
+#pragma unroll
+  for (int i = 1; i < kJoinGroups; ++i) {
+    const float4 x = sums[i][lane];
+    o[0] += x.x;
+    o[1] += x.y;
+    o[2] += x.z;
+    o[3] += x.w;
+  }
+  write_item<T, D, NT>(a, b, seg, item, o);
 }
 
 // Query rows per tile: 8 NT.
@@ -788,26 +972,61 @@ constexpr int64_t kOneLaunchLen = 512;
 
 inline bool one_launch(const ml_kv8_cache* c) { return c->max_len <= kOneLaunchLen; }
 
-template <typename T, int FMT, int D, int NT>
-int launch(AttnArgs a, cudaStream_t st) {
-  using C = Config<D, NT>;
-  auto kernel = kv8_attention_kernel<T, FMT, D, NT>;
+// CTAs of the list: two waves of two per SM, which even out what one wave
+// leaves (CTAs with equal runs differ by up to a quarter in time), one where
+// there is too little work for that.
+inline int ctas_of_list(const ml_kv8_cache* c, int64_t row_tiles, int warps) {
+  const int one = 2 * num_sms();
+  const int64_t most = c->batch * c->kv_heads * row_tiles * (c->max_len / kTile + kPad);
+  const int ctas = most >= (int64_t)one * warps * 16 ? 2 * one : one;
+  return ctas < kMaxCtas ? ctas : kMaxCtas;
+}
+
+struct Plan {
+  int nt, row_tiles, ctas;
+  size_t workspace;
+};
+inline Plan plan_of(const ml_kv8_cache* c, int64_t rows) {
+  Plan p;
+  p.nt = n_tiles(rows, c->head_dim);
+  p.row_tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+  const int warps = list_warps((int)c->head_dim, p.nt);
+  p.ctas = ctas_of_list(c, p.row_tiles, warps);
+  const int64_t piece = p.nt * c->head_dim / 16 * 4 * 32 + 3 * 8 * p.nt;
+  p.workspace = one_launch(c) ? 0 : (size_t)p.ctas * (2 + warps) * piece * sizeof(float);
+  return p;
+}
+
+template <typename T, int FMT, int D, int NT, int NW>
+int launch_kernel(const AttnArgs& a, int64_t grid, cudaStream_t st) {
+  using C = Config<D, NT, NW>;
+  auto kernel = kv8_attention_kernel<T, FMT, D, NT, NW>;
   static PerDevice<cudaError_t> attr;
   ML_CHECK_CUDA(attr.get([&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 (int)C::smem());
   }), "kv8_attention");
-  const int64_t segs = (int64_t)a.batch * a.kv_heads * a.row_tiles;
-  ML_CHECK_ARG(segs < ((int64_t)1 << 31), "kv8_attention: too many rows");
-  const dim3 grid((unsigned)(a.part ? a.ctas : segs));
-  ML_CHECK_CUDA(launch_pdl(kernel, grid, dim3(32 * C::kWarps), C::smem(), st, a),
+  ML_CHECK_CUDA(launch_pdl(kernel, dim3((unsigned)grid), dim3(32 * NW), C::smem(), st, a),
                 "kv8_attention");
-  if (a.part) {
-    const int64_t chunks = ((int64_t)a.kv_heads * a.row_tiles + 3) / 4;
-    ML_CHECK_CUDA(launch_pdl(kv8_attention_join<T, D, NT>, dim3((unsigned)(a.batch * chunks)),
-                             dim3(128), 0, st, a),
-                  "kv8_attention(join)");
-  }
+  return ML_OK;
+}
+
+template <typename T, int FMT, int D, int NT>
+int launch(AttnArgs a, cudaStream_t st) {
+  const int64_t segs = (int64_t)a.batch * a.kv_heads * a.row_tiles;
+  ML_CHECK_ARG(segs * (a.max_len / kTile + kPad) < ((int64_t)1 << 31),
+               "kv8_attention: too many query rows for this cache in one call");
+  if (a.part == nullptr)
+    return launch_kernel<T, FMT, D, NT, segment_warps(D, NT)>(a, segs, st);
+  constexpr int NW = list_warps(D, NT);
+  const int rc = launch_kernel<T, FMT, D, NT, NW>(a, a.ctas, st);
+  if (rc != ML_OK) return rc;
+  const int64_t parts = Config<D, NT, NW>::kImage / 4 / 32;
+  a.split = segs * parts <= 4 * num_sms();
+  ML_CHECK_CUDA(launch_pdl(kv8_attention_join<T, D, NT, NW>,
+                           dim3((unsigned)(a.split ? segs * parts : segs)), dim3(kJoinThreads), 0,
+                           st, a),
+                "kv8_attention(join)");
   return ML_OK;
 }
 
@@ -825,12 +1044,9 @@ using namespace ml;
 
 extern "C" size_t ml_kv8_attention_workspace_bytes(const ml_kv8_cache* cache, int64_t q_heads,
                                                    int64_t tokens) {
-  if (cache == nullptr || cache->kv_heads <= 0 || cache->batch <= 0 || tokens <= 0 ||
-      q_heads <= 0 || one_launch(cache))
+  if (cache == nullptr || cache->kv_heads <= 0 || cache->batch <= 0 || tokens <= 0 || q_heads <= 0)
     return 0;
-  const int nt = n_tiles(q_heads / cache->kv_heads * tokens, cache->head_dim);
-  const int64_t piece = nt * cache->head_dim / 16 * 4 * 32 + 3 * 8 * nt;
-  return (size_t)num_sms() * 2 * piece * sizeof(float);
+  return plan_of(cache, q_heads / cache->kv_heads * tokens).workspace;
 }
 
 extern "C" int ml_kv8_attention(const ml_kv8_cache* cache, const void* q, const int64_t* q_strides,
@@ -852,8 +1068,11 @@ extern "C" int ml_kv8_attention(const ml_kv8_cache* cache, const void* q, const 
   ML_CHECK_ARG(aligned16(q) && aligned16(out), "kv8_attention: q and out must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     ML_CHECK_ARG(q_strides[i] % 8 == 0, "kv8_attention: q strides must be multiples of 8 elements");
-  const size_t need = ml_kv8_attention_workspace_bytes(cache, q_heads, tokens);
-  ML_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+  const int64_t rows = q_heads / cache->kv_heads * tokens;
+  ML_CHECK_ARG(rows < ((int64_t)1 << 30), "kv8_attention: too many rows");
+  const Plan plan = plan_of(cache, rows);
+  ML_CHECK_ARG(plan.workspace == 0 ||
+                   (workspace && aligned16(workspace) && workspace_bytes >= plan.workspace),
                "kv8_attention: workspace too small");
   AttnArgs a;
   a.q = q;
@@ -866,17 +1085,16 @@ extern "C" int ml_kv8_attention(const ml_kv8_cache* cache, const void* q, const 
   a.batch = (int)cache->batch;
   a.kv_heads = (int)cache->kv_heads;
   a.group = (int)(q_heads / cache->kv_heads);
-  const int64_t rows = a.group * tokens;
-  ML_CHECK_ARG(rows < ((int64_t)1 << 30), "kv8_attention: too many rows");
-  const int nt = n_tiles(rows, cache->head_dim);
   a.rows = (int)rows;
-  a.row_tiles = (int)((rows + 8 * nt - 1) / (8 * nt));
+  a.row_tiles = plan.row_tiles;
   a.max_len = (int)cache->max_len;
   a.block = (int)cache->block;
+  a.tiles_log2 = a.block == 32 ? 0 : a.block == 64 ? 1 : 2;
   a.qk_scale = scale * 1.4426950408889634f;
   a.out = out;
-  a.part = need ? static_cast<float*>(workspace) : nullptr;
-  a.ctas = num_sms();
+  a.part = plan.workspace ? static_cast<float*>(workspace) : nullptr;
+  a.ctas = plan.ctas;
+  const int nt = plan.nt;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == ML_DTYPE_BF16;
   if (cache->format == ML_KV8_INT8)

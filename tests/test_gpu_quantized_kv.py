@@ -261,6 +261,15 @@ def test_attention_of_a_block_that_reads_as_nan():
     out = quantized_kv_attention(q, kv, torch.tensor([127], device=DEV))      # sees 128, 129
     assert torch.isfinite(out[0, 0]).all() and torch.isfinite(out[0, 1, :2]).all()
     assert torch.isnan(out[0, 1, 2:]).all()
+    # the poisoned block alone, seen by one warp, and by several CTAs
+    for L2, n in ((64, 30), (4096, 4000)):
+        one = allocate_quantized_kv(1, 1, L2, D, "fp8", torch.bfloat16, 32)
+        rows = torch.zeros(1, 1, n, D, dtype=torch.bfloat16)
+        rows[..., n - 1, 5] = float("inf")
+        quantized_kv_append(one, torch.zeros_like(rows).to(DEV), rows.to(DEV),
+                            torch.zeros(1, dtype=torch.int64, device=DEV))
+        out = quantized_kv_attention(q[:, :1, :1], one, torch.tensor([n - 1], device=DEV))
+        assert torch.isnan(out).all()
     k[0, 0, 199, 0] = float("inf")
     quantized_kv_append(kv, k.to(DEV), v.to(DEV), torch.zeros(1, dtype=torch.int64, device=DEV))
     out = quantized_kv_attention(q, kv, torch.tensor([199], device=DEV))

@@ -83,17 +83,21 @@ constexpr int segment_warps(int D, int NT) { return 2 * list_warps(D, NT); }
 // The flat list of tiles
 // ---------------------------------------------------------------------------
 
+// Positions that query t of sequence b sees.  (start and count are loaded
+// together: the second does not wait for the first.)
 __device__ __forceinline__ int visible(const AttnArgs& a, int b, int t) {
-  if (t >= a.span.count(b)) return 0;
-  const int64_t n = a.span.first(b) + t + 1;
-  return n <= 0 ? 0 : n > a.max_len ? a.max_len : (int)n;
+  const int64_t start = a.span.first(b);
+  const int count = a.span.count(b);
+  const int64_t n = start + t + 1;
+  return t >= count || n <= 0 ? 0 : n > a.max_len ? a.max_len : (int)n;
 }
 // Tiles of each segment of sequence b: up to its last real query's position,
 // at least one (which then writes the zeros).
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) {
-  const int c = a.span.count(b);
-  const int n = c > 0 ? visible(a, b, c - 1) : 0;
-  return n <= 0 ? 1 : (n + kTile - 1) / kTile;
+  const int64_t start = a.span.first(b);
+  const int count = a.span.count(b);
+  const int64_t n = count > 0 ? start + count : 0;
+  return n <= 0 ? 1 : ((n > a.max_len ? a.max_len : (int)n) + kTile - 1) / kTile;
 }
 __device__ __forceinline__ int tiles_per_cta(int total, int ctas, int warps) {
   const int even = (int)(((unsigned)total + ctas - 1) / (unsigned)ctas);

@@ -15,18 +15,24 @@
 //
 // A choice at a border must not depend on the order of a sum, so weights are
 // summed as integers: W = round(2^43 w), which keeps V <= 2^20 of them below
-// 2^63 and is exact in any order.  Where w < e^-17 it comes from the fp32
-// exponential (off by under 2^-19 of it, which is 2^-43 of the largest), above
-// from the fp64 one.
+// 2^63 and is exact in any order.  Where w < 2^-24.5 it comes from the fp32
+// exponential (off by under 2^-18 of it, so by 2^-42 of the largest at most),
+// above from fp64: 2^(i/256) from a table times a quartic in the rest, |r| <=
+// 2^-9, good to 2^-50.
 //
 // A cluster of CTAs holds a row in shared memory, so HBM is read once; every
 // step is then a pass over the CTA's slice and an exchange of a few words
 // through distributed shared memory.  The kept set is a prefix of the order and
 // is found by selection, not by sorting: a histogram over the distance to the
 // largest logit, of counts (top-k) or weights (top-p), gives the bin that the
-// prefix ends in, histograms over that bin's keys narrow it to one key (one or
-// two more for 16-bit logits), and the tokens equal to that key are cut by
-// index.  The draw adds up kept weights by CTA, warp and lane in index order.
+// prefix ends in.  The tokens from there up are few as a rule; they go, in
+// index order, to a list in the cluster's first CTA, which finishes alone.
+// Otherwise the steps go on over the slices.  Histograms over the bin's keys
+// narrow it to one key, the tokens equal to it are cut by index, and the draw
+// adds up kept weights by CTA, warp and lane in index order.
+//
+// Tokens that need fp64 are rare in most rows and everywhere in flat ones: a
+// warp queues them and weighs 32 at a time.
 #include "common.cuh"
 
 #include <cooperative_groups.h>
@@ -43,7 +49,10 @@ constexpr int kMaxCluster = 16;
 constexpr int kMaxSlice = 65536;     // tokens of a CTA: the histogram's 32-bit parts hold them
 constexpr int64_t kMaxVocab = (int64_t)1 << 20;
 constexpr double kOne = 8796093022208.0;  // 2^43
-constexpr size_t kMaxResident = 200 * 1024;
+constexpr size_t kMaxResident = 160 * 1024;
+constexpr int kList = 1024;          // tokens of the list
+constexpr int kWarpList = kList / kWarps;  // of them from one warp
+constexpr int kTable = 256;
 
 struct SampleArgs {
   const void* logits;  // [rows, V] at row pitch ld
@@ -74,43 +83,69 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 
 // What the weights and bins of a row are computed with.
 struct Row {
-  uint32_t top_key;
-  float top, inv_t_f;
-  double inv_t;
+  float top;
+  float rate_f;      // log2(e) / t
+  double inv_t, rate;
+  const double* table;
 
+  // log2 of the weight, in fp32: NaN at the top itself where the rate or the
+  // top is infinite
+  __device__ __forceinline__ float log2_weight(float x) const { return (x - top) * rate_f; }
+  __device__ __forceinline__ static bool small(float z) { return z < -24.5f; }
+  __device__ __forceinline__ static uint32_t small_weight(float z) {
+    // 2^43 2^z < 2^19, rounded by adding 2^23
+    float w;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
+    return __float_as_uint(fmaf(w, (float)kOne, 8388608.f)) - 0x4b000000u;
+  }
+  __device__ __forceinline__ uint64_t large_weight(float x) const {
+    if (x == top) return (uint64_t)kOne;
+    const double y = ((double)x - (double)top) * rate;
+    const double magic = 26388279066624.0;  // 1.5 * 2^44: its steps are 2^-8
+    const double shifted = y + magic;
+    const int k = __double2loint(shifted);
+    const double r = y - (shifted - magic);
+    // 2^r - 1
+    const double p = r * fma(r, fma(r, fma(r, 0.009618129107628477, 0.05550410866482158),
+                                    0.24022650695910072), 0.6931471805599453);
+    const double t = table[k & (kTable - 1)];
+    double w = fma(t, p, t);
+    w = __hiloint2double(__double2hiint(w) + ((k >> 8) << 20), __double2loint(w));
+    const double i = fma(w, kOne, 4503599627370496.0);  // + 2^52: the integer in its low bits
+    return (uint64_t)__double_as_longlong(i) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    const float z = log2_weight(x);
+    return small(z) ? small_weight(z) : large_weight(x);
+  }
   __device__ __forceinline__ double exact(float x) const {
     return x == top ? 1.0 : exp(((double)x - (double)top) * inv_t);
   }
-  __device__ __forceinline__ uint64_t weight(float x) const {
-    if (x == top) return (uint64_t)kOne;  // also where both are +inf
-    const float z = (x - top) * inv_t_f;
-    if (!(z >= -31.f)) return 0;  // under half of 2^-43 (or x far below a top of +inf)
-    if (z < -17.f) return __float2uint_rn(__expf(z) * (float)kOne);
-    return (uint64_t)__double2ll_rn(exact(x) * kOne);
-  }
 };
 
-// Which tokens an earlier cut has left: key > cut, or equal and index < end.
+// Which tokens are left: logit > x, or equal and index < end.  (NaN never is.)
 struct Cut {
-  uint32_t key = 0;
+  float x = -INFINITY;
   int end = 0;
-  __device__ __forceinline__ bool has(uint32_t k, int i) const {
-    return k > key || (k == key && i < end && k != 0);
-  }
+  __device__ __forceinline__ bool has(float v, int i) const { return v > x || (v == x && i < end); }
 };
 
 struct Shared {
+  double table[kTable];            // 2^(i / kTable)
   uint32_t hist[2][3][kBins];      // 15-bit parts of the sums, two in turn
   uint64_t sums[kBins];            // over the cluster
-  uint64_t slot[8][kMaxCluster];   // one exchange each
+  uint64_t slot[10][kMaxCluster];  // one exchange each
   uint64_t part[kWarps];
   uint64_t above;
   int bin, found;
   uint32_t key[2];
+  float queue[kWarps][64];
+  float list_x[kList];
+  int list_i[kList];
 };
 
-// A CTA's view of its slice: `vec(v)` is 16-byte vector v of the slice, whose
-// first token has index `base + v * N`; tokens outside the row read as -inf.
+// A CTA's view of its slice: `get(v, x)` gives the N tokens of 16-byte vector v,
+// the first of which has index `index(v)`; tokens outside the row read as -inf.
 template <typename T>
 struct Slice {
   static constexpr int N = 16 / sizeof(T);
@@ -127,32 +162,99 @@ struct Slice {
       r.v[e] = i + e >= 0 && i + e < V ? row[i + e] : from_f32<T>(-INFINITY);
     return r;
   }
-  __device__ __forceinline__ Vec16<T> vec(int v) const {
-    if (held == nullptr) return fetch(v);
+  __device__ __forceinline__ void get(int v, float* x) const {
     Vec16<T> r;
-    *reinterpret_cast<uint4*>(&r) = held[v];
-    return r;
-  }
-  // Calls f(x, key, index) for the tokens of this warp's share of the slice;
-  // lanes interleave by vector, so a lane's tokens ascend.
-  template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-    const int per = (count + kWarps - 1) / kWarps, warp = threadIdx.x >> 5;
-    const int end = min(count, (warp + 1) * per);
-    for (int v = warp * per + (threadIdx.x & 31); v < end; v += 32) {
-      const Vec16<T> r = vec(v);
+    if (held == nullptr) r = fetch(v);
+    else *reinterpret_cast<uint4*>(&r) = held[v];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float x = to_f32(r.v[e]);
-        f(x, key_of(x), base + v * N + e);
+    for (int e = 0; e < N; ++e) x[e] = to_f32(r.v[e]);
+  }
+  __device__ __forceinline__ int index(int v) const { return base + v * N; }
+};
+// The list, a token at a time.
+struct List {
+  static constexpr int N = 1;
+  const float* x_;
+  const int* i_;
+  int count;
+  __device__ __forceinline__ void get(int v, float* x) const { x[0] = x_[v]; }
+  __device__ __forceinline__ int index(int v) const { return i_[v]; }
+};
+
+// Calls f(active, x[N], index) for the tokens of this warp's share of the
+// source, all lanes together; lanes interleave, so a lane's tokens ascend.
+template <typename S, typename F>
+__device__ __forceinline__ void each(const S& src, F&& f) {
+  const int per = (src.count + kWarps - 1) / kWarps, warp = threadIdx.x >> 5;
+  const int begin = warp * per, end = min(src.count, begin + per);
+  for (int v0 = begin; v0 < end; v0 += 32) {
+    const int v = v0 + (threadIdx.x & 31);
+    float x[S::N];
+    int i = 0;
+    if (v < end) {
+      src.get(v, x);
+      i = src.index(v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < S::N; ++e) x[e] = -INFINITY;
+    }
+    f(x, i);
+  }
+}
+
+// each() for weights: sink(x, W, valid) gets the large ones, a warp at a time;
+// the sum of this lane's small ones is returned.
+template <typename S, typename F>
+__device__ __forceinline__ uint64_t each_weight(const S& src, const Row& row, const Cut& cut,
+                                                float* queue, F&& sink) {
+  const int lane = threadIdx.x & 31;
+  const unsigned before = (1u << lane) - 1;
+  uint64_t tail = 0;
+  int waiting = 0, at = 0;
+  each(src, [&](const float* x, int i) {
+    uint32_t small = 0;
+#pragma unroll
+    for (int e = 0; e < S::N; ++e) {
+      const float z = row.log2_weight(x[e]);
+      const bool in = cut.has(x[e], i + e), little = Row::small(z);
+      if (in && little) small += Row::small_weight(z);
+      const unsigned m = __ballot_sync(0xffffffffu, in && !little);
+      if (m) {
+        if (in && !little) queue[(at + waiting + __popc(m & before)) & 63] = x[e];
+        waiting += __popc(m);
+        if (waiting >= 32) {
+          __syncwarp();
+          const float q = queue[(at + lane) & 63];
+          __syncwarp();
+          at += 32;
+          waiting -= 32;
+          sink(q, row.large_weight(q), true);
+        }
       }
     }
+    tail += small;
+  });
+  __syncwarp();
+  if (waiting) {
+    const float q = lane < waiting ? queue[(at + lane) & 63] : row.top;
+    sink(q, row.large_weight(q), lane < waiting);
   }
-};
+  __syncwarp();
+  return tail;
+}
 
 __device__ __forceinline__ uint64_t warp_sum64(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ uint64_t warp_scan64(uint64_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t c = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += c;
+  }
   return v;
 }
 
@@ -173,47 +275,39 @@ struct Cluster {
   }
 };
 
-// Adds to one bin at a time, runs of equal bins in a register.
-struct Adder {
-  uint32_t (*hist)[kBins];
-  int bin = -1;
-  uint64_t sum = 0;
-
-  __device__ __forceinline__ void flush() {
-    if (bin < 0) return;
-    const uint32_t lo = (uint32_t)sum & 0x7fff, mid = (uint32_t)(sum >> 15) & 0x7fff,
-                   hi = (uint32_t)(sum >> 30);
-    if (lo) atomicAdd(&hist[0][bin], lo);
-    if (mid) atomicAdd(&hist[1][bin], mid);
-    if (hi) atomicAdd(&hist[2][bin], hi);
+__device__ __forceinline__ void add_parts(uint32_t (*hist)[kBins], int bin, uint64_t v) {
+  const uint32_t lo = (uint32_t)v & 0x7fff, mid = (uint32_t)(v >> 15) & 0x7fff,
+                 hi = (uint32_t)(v >> 30);
+  if (lo) atomicAdd(&hist[0][bin], lo);
+  if (mid) atomicAdd(&hist[1][bin], mid);
+  if (hi) atomicAdd(&hist[2][bin], hi);
+}
+// The same from a whole warp, which often has one bin (flat rows, the far end).
+__device__ __forceinline__ void add_warp(uint32_t (*hist)[kBins], int bin, uint64_t v, bool valid) {
+  const int b0 = __shfl_sync(0xffffffffu, bin, 0);
+  if (__all_sync(0xffffffffu, !valid || bin == b0)) {
+    v = warp_sum64(valid ? v : 0);
+    if ((threadIdx.x & 31) == 0) add_parts(hist, b0, v);
+  } else if (valid) {
+    add_parts(hist, bin, v);
   }
-  __device__ __forceinline__ void add(int b, uint64_t v) {
-    if (b == bin) {
-      sum += v;
-    } else {
-      flush();
-      bin = b;
-      sum = v;
-    }
-  }
-};
+}
 
-// The first index past the `want`-th token (in index order) of those that
-// `value` counts, or past the first whose running sum exceeds `want` (OVER):
-// by CTA, then warp, then lane.  Returns that token's index in every CTA; -1
-// where the values do not reach that far.  `total`: the sum over the cluster.
-template <bool OVER, typename T, typename F>
-__device__ int locate(const Slice<T>& sl, const Cluster& cl, Shared& sh, int step, double want,
-                      F&& value, uint64_t* total_out, double (*want_of)(uint64_t, double)) {
+// What the draw and the cut by index share: `mine` is the sum of this warp's
+// share of the source, value(x, i) that of one token.  Finds the first token, in
+// index order, at which the running sum over the cluster passes `want` (OVER) or
+// reaches it.  Returns its index in the CTA that has it, -1 in the others and
+// where the sum does not get there.  FRACTION: want is a fraction of the total.
+template <bool OVER, bool FRACTION, typename S, typename F>
+__device__ int locate(const S& src, const Cluster& cl, Shared& sh, int step, double want,
+                      uint64_t mine, F&& value, uint64_t* total_out) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint64_t mine = 0;
-  sl.each([&](float x, uint32_t key, int i) { mine += value(x, key, i); });
-  mine = warp_sum64(mine);
   __syncthreads();
   if (lane == 0) sh.part[warp] = mine;
   if (threadIdx.x == 0) sh.found = -1;
   __syncthreads();
   uint64_t here = 0, upto = 0;  // of the CTA, before this warp
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) upto += sh.part[w];
     here += sh.part[w];
@@ -225,38 +319,35 @@ __device__ int locate(const Slice<T>& sl, const Cluster& cl, Shared& sh, int ste
     total += sh.slot[step][r];
   }
   *total_out = total;
-  const double target = want_of(total, want);
+  const double target = FRACTION ? want * (double)total : want;
   auto reached = [&](uint64_t s) { return OVER ? (double)s > target : (double)s >= target; };
   uint64_t run = before + upto;
   if (mine > 0 && !reached(run) && reached(run + mine)) {
     // one warp of the cluster: walk its share
-    const int per = (sl.count + kWarps - 1) / kWarps, end = min(sl.count, (warp + 1) * per);
+    const int per = (src.count + kWarps - 1) / kWarps, end = min(src.count, (warp + 1) * per);
     for (int v0 = warp * per; v0 < end; v0 += 32) {
       const int v = v0 + lane;
-      uint64_t w[Slice<T>::N], s = 0;
-      Vec16<T> r;
-      if (v < end) r = sl.vec(v);
-#pragma unroll
-      for (int e = 0; e < Slice<T>::N; ++e) {
-        const float x = to_f32(r.v[e]);
-        w[e] = v < end ? value(x, key_of(x), sl.base + v * Slice<T>::N + e) : 0;
-        s += w[e];
+      float x[S::N];
+      uint64_t s = 0;
+      int i = 0;
+      if (v < end) {
+        src.get(v, x);
+        i = src.index(v);
+#pragma unroll 1
+        for (int e = 0; e < S::N; ++e) s += value(x[e], i + e);
       }
-      uint64_t incl = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t c = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += c;
-      }
+      const uint64_t incl = warp_scan64(s);
       uint64_t at = run + incl - s;
       const bool hit = s > 0 && !reached(at) && reached(at + s);
       if (hit) {
-        for (int e = 0; e < Slice<T>::N; ++e) {
-          if (w[e] > 0 && reached(at + w[e])) {
-            sh.found = sl.base + v * Slice<T>::N + e;
+#pragma unroll 1
+        for (int e = 0; e < S::N; ++e) {
+          const uint64_t w = value(x[e], i + e);
+          if (w > 0 && reached(at + w)) {
+            sh.found = i + e;
             break;
           }
-          at += w[e];
+          at += w;
         }
       }
       if (__any_sync(0xffffffffu, hit)) break;
@@ -267,133 +358,305 @@ __device__ int locate(const Slice<T>& sl, const Cluster& cl, Shared& sh, int ste
   return sh.found;
 }
 
-// The prefix of the tokens in `in` whose values (counts or weights) first
-// reach `need` (WEIGHT: p of their sum), as a cut.
-template <bool WEIGHT, typename T>
-__device__ Cut select(const Slice<T>& sl, const Cluster& cl, Shared& sh, const Row& row,
-                      const Cut& in, bool all, uint64_t need, double p, int step, int& round) {
+// Where a selection stands: the prefix ends among the keys [lo, hi], after
+// values of `above` before them; `need` in all.
+struct Search {
+  uint32_t lo, hi;
+  uint64_t above, need;
+  int round;    // histograms so far (of the two in turn)
+  bool whole;   // nothing to cut
+};
+
+// One histogram of the tokens in `in` and [q.lo, q.hi], by distance to the top
+// (first = true) or by key; q narrows to the bin that the prefix ends in.
+// WEIGHT: q.need becomes p of the sum, on the first call with all tokens.
+template <bool WEIGHT, typename S>
+__device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const Row& row, const Cut& in,
+                       Search& q, bool first, double p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // counts: bins of 1/16 over 32; weights: of 1/32 over 16, in units of t
-  const float per = WEIGHT ? row.inv_t_f * 32.f : 16.f;
+  // counts: bins of 1/16 over 32; weights: of 1/32 over 16, in units of log2
+  const float per = WEIGHT ? row.rate_f * 32.f : 16.f;
   auto distance = [&](float x) { return min(__float2int_rz((row.top - x) * per), kBins - 1); };
-  uint32_t lo = kLowest, hi = row.top_key;  // the keys still in question
-  uint64_t above = 0;
-  int shift = -1;                     // -1: bins of distance
-  while (true) {
-    uint32_t (*hist)[kBins] = sh.hist[round & 1];
-    ++round;
+  const int bits = 32 - __clz(q.hi - q.lo);
+  const int shift = bits > 9 ? bits - 9 : 0;
+  auto bin_of = [&](float x) { return first ? distance(x) : (int)((q.hi - key_of(x)) >> shift); };
+  uint32_t (*hist)[kBins] = sh.hist[q.round & 1];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) hist[i][tid] = 0;
-    __syncthreads();
-    Adder add{hist};
-    sl.each([&](float x, uint32_t key, int i) {
-      if (key < lo || key > hi || !(all || in.has(key, i))) return;
-      const uint64_t v = WEIGHT ? row.weight(x) : 1;
-      if (v) add.add(shift < 0 ? distance(x) : (int)((hi - key) >> shift), v);
+  for (int i = 0; i < 3; ++i) hist[i][tid] = 0;
+  __syncthreads();
+  // keys and logits have the same order
+  const float x_lo = value_of(q.lo), x_hi = value_of(q.hi);
+  if (WEIGHT && first) {
+    uint64_t tail = each_weight(src, row, in, sh.queue[warp], [&](float x, uint64_t w, bool valid) {
+      add_warp(hist, distance(x), w, valid);
     });
-    add.flush();
-    cl.sync();
-    {
-      // a thread per bin of this CTA's share and CTA that counted it
-      const int r = tid % cl.size, bin = cl.rank * (kBins / cl.size) + tid / cl.size;
-      const Shared* o = cl.of(&sh, r);
-      const uint32_t (*h)[kBins] = o->hist[(round - 1) & 1];
-      uint64_t v = h[0][bin] + ((uint64_t)h[1][bin] << 15) + ((uint64_t)h[2][bin] << 30);
-      for (int o2 = cl.size / 2; o2 > 0; o2 >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o2);
-      cl.of(&sh, r)->sums[bin] = v;
-    }
-    if (tid == 0) sh.bin = -1;
-    cl.sync();
-    const uint64_t s = sh.sums[tid];
-    uint64_t incl = s;
+    tail = warp_sum64(tail);  // all of them lie in the last bin, or rate * 32 overflows
+    if (lane == 0) add_parts(hist, kBins - 1, tail);
+  } else {
+    each(src, [&](const float* x, int i) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t c = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += c;
-    }
-    if (lane == 31) sh.part[warp] = incl;
-    __syncthreads();
-    uint64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) incl += sh.part[w];
-      total += sh.part[w];
-    }
-    if (shift < 0) {
-      if (WEIGHT) {
-        const double f = ceil(p * (double)total);
-        need = f < 1.0 ? 1 : (uint64_t)f;
-      }
-      if (need >= total) {  // nothing to cut, or by rounding all of it
-        Cut c = in;
-        if (all) {
-          c.key = 1;
-          c.end = 0x7fffffff;
+      for (int e = 0; e < S::N; ++e)
+        if (x[e] >= x_lo && x[e] <= x_hi && in.has(x[e], i + e)) {
+          if (WEIGHT) add_parts(hist, bin_of(x[e]), row.weight(x[e]));
+          else atomicAdd(&hist[0][bin_of(x[e])], 1u);
         }
-        return c;
-      }
-    }
-    if (above + incl >= need && above + incl - s < need) {
-      sh.bin = tid;
-      sh.above = above + incl - s;
-    }
-    __syncthreads();
-    const int bin = sh.bin;
-    above = sh.above;
-    __syncthreads();
-    if (shift < 0) {
-      // The keys of a bin of distances are neighbours: find the first and last
-      // (distances fall as keys grow) by 32-way search, a warp for each.
-      if (warp < 2) {
-        // smallest key in [lo, hi] with distance <= bin (warp 0) / < bin (warp 1)
-        uint32_t a = lo, b = hi + 1;  // the answer lies in [a, b]
-        while (a < b) {
-          const uint32_t step_k = (b - a + 31) / 32;
-          const uint64_t k = (uint64_t)a + (uint64_t)step_k * lane;
-          bool ok = k >= b;
-          if (!ok) {
-            const int d = distance(value_of((uint32_t)k));
-            ok = warp == 0 ? d <= bin : d < bin;
-          }
-          const unsigned m = __ballot_sync(0xffffffffu, ok);
-          const int f = m ? __ffs(m) - 1 : 32;
-          const uint64_t top_k = (uint64_t)a + (uint64_t)step_k * f;
-          const uint32_t nb = top_k < b ? (uint32_t)top_k : b;
-          const uint32_t na = f == 0 ? a : (uint32_t)((uint64_t)a + (uint64_t)step_k * (f - 1) + 1);
-          a = f == 0 ? nb : na;
-          b = nb;
-        }
-        if (lane == 0) sh.key[warp] = a;
-      }
-      __syncthreads();
-      lo = sh.key[0];
-      hi = sh.key[1] - 1;
-      __syncthreads();
-    } else {
-      const uint32_t h = hi - ((uint32_t)bin << shift);
-      const uint32_t span = (1u << shift) - 1;
-      lo = h - lo > span ? h - span : lo;
-      hi = h;
-    }
-    if (lo == hi) break;
-    const int bits = 32 - __clz(hi - lo);
-    shift = bits > 9 ? bits - 9 : 0;
+    });
   }
-  // the tokens equal to the key: as many as are still needed, lowest index first
-  const uint64_t each = WEIGHT ? row.weight(value_of(lo)) : 1;
-  const uint64_t want = (need - above + each - 1) / each;
-  uint64_t ties;
-  const int at = locate<false>(
-      sl, cl, sh, step, (double)want,
-      [&](float, uint32_t key, int i) -> uint64_t { return key == lo && (all || in.has(key, i)); },
-      &ties, [](uint64_t, double w) { return w; });
-  // (every CTA learns it: only one found it)
+  cl.sync();
+  {
+    // a thread per bin of this CTA's share and CTA that counted it
+    const int r = tid % cl.size, bin = cl.rank * (kBins / cl.size) + tid / cl.size;
+    const uint32_t (*h)[kBins] = cl.of(&sh, r)->hist[q.round & 1];
+    uint64_t v = h[0][bin] + ((uint64_t)h[1][bin] << 15) + ((uint64_t)h[2][bin] << 30);
+    for (int o = cl.size / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    cl.of(&sh, r)->sums[bin] = v;
+  }
+  ++q.round;
+  if (tid == 0) sh.bin = kBins - 1;
+  cl.sync();
+  const uint64_t s = sh.sums[tid];
+  uint64_t incl = warp_scan64(s);
+  if (lane == 31) sh.part[warp] = incl;
+  __syncthreads();
+  uint64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) incl += sh.part[w];
+    total += sh.part[w];
+  }
+  if (first) {
+    if (WEIGHT && q.need == 0) {
+      const double f = ceil(p * (double)total);
+      q.need = f < 1.0 ? 1 : (uint64_t)f;
+    }
+    if (q.need >= total) {
+      q.whole = true;
+      return;
+    }
+  }
+  if (q.above + incl >= q.need && q.above + incl - s < q.need) {
+    sh.bin = tid;
+    sh.above = q.above + incl - s;
+  }
+  __syncthreads();
+  const int bin = sh.bin;
+  q.above = sh.above;
+  if (!first) {
+    const uint64_t down = (uint64_t)bin << shift;
+    const uint32_t h = down <= q.hi - q.lo ? q.hi - (uint32_t)down : q.lo;
+    const uint32_t span = (1u << shift) - 1;
+    q.lo = h - q.lo > span ? h - span : q.lo;
+    q.hi = h;
+    return;
+  }
+  // The keys of a bin of distances are neighbours: find the first and last
+  // (distances fall as keys grow) by 32-way search, a warp for each: the
+  // smallest key with a distance <= bin, and < bin.
+  if (warp < 2) {
+    uint32_t a = q.lo, b = q.hi + 1;  // the answer lies in [a, b]
+    while (a < b) {
+      const uint32_t step = (b - a + 31) / 32;
+      const uint64_t k = (uint64_t)a + (uint64_t)step * lane;
+      bool ok = k >= b;
+      if (!ok) {
+        const int d = distance(value_of((uint32_t)k));
+        ok = warp == 0 ? d <= bin : d < bin;
+      }
+      const unsigned m = __ballot_sync(0xffffffffu, ok);
+      const int f = m ? __ffs(m) - 1 : 32;
+      const uint64_t t = (uint64_t)a + (uint64_t)step * f;
+      const uint32_t nb = t < b ? (uint32_t)t : b;
+      a = f == 0 ? nb : (uint32_t)((uint64_t)a + (uint64_t)step * (f - 1) + 1);
+      b = nb;
+    }
+    if (lane == 0) sh.key[warp] = a;
+  }
+  __syncthreads();
+  q.lo = sh.key[0];
+  q.hi = sh.key[1] - 1;
+}
+
+// Narrows to one key and cuts the tokens equal to it by index.
+template <bool WEIGHT, typename S>
+__device__ Cut finish(const S& src, const Cluster& cl, Shared& sh, const Row& row, const Cut& in,
+                      Search& q, int step) {
+  while (q.lo < q.hi) narrow<WEIGHT>(src, cl, sh, row, in, q, false, 0.0);
+  // as many as are still needed, lowest index first
+  const float x = value_of(q.lo);
+  const uint64_t each_w = WEIGHT ? row.weight(x) : 1;
+  const uint64_t want = (q.need - q.above + each_w - 1) / each_w;
+  auto value = [&](float v, int i) -> uint64_t { return v == x && in.has(v, i); };
+  uint64_t mine = 0, ties;
+  each(src, [&](const float* v, int i) {
+#pragma unroll
+    for (int e = 0; e < S::N; ++e) mine += value(v[e], i + e);
+  });
+  mine = warp_sum64(mine);
+  const int at = locate<false, false>(src, cl, sh, step, (double)want, mine, value, &ties);
+  // one CTA found it, all learn it
   cl.gather(sh, step + 1, (uint64_t)(int64_t)at);
   Cut c;
-  c.key = lo;
-  c.end = 0;
+  c.x = x;
   for (int r = 0; r < cl.size; ++r) c.end = max(c.end, (int)(int64_t)sh.slot[step + 1][r] + 1);
   return c;
+}
+
+// The tokens with a logit >= x, in index order, to the first CTA's list;
+// returns their number there and everywhere, or -1 where they do not fit.
+template <typename T>
+__device__ int collect(const Slice<T>& sl, const Cluster& cl, Shared& sh, float x) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // each warp's go to a stretch of this CTA's own (idle) list space, the first
+  // CTA's first warps' included: they are moved once all are counted
+  int n = 0;
+  constexpr int kHold = kWarpList;
+  float* hx = sh.list_x + warp * kHold;
+  int* hi = sh.list_i + warp * kHold;
+  each(sl, [&](const float* v, int i) {
+    unsigned mask = 0;
+#pragma unroll
+    for (int e = 0; e < Slice<T>::N; ++e)
+      if (v[e] >= x) mask |= 1u << e;
+    if (!__any_sync(0xffffffffu, mask != 0)) return;
+    const int c = __popc(mask);
+    int incl = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    int at = n + incl - c;
+#pragma unroll
+    for (int e = 0; e < Slice<T>::N; ++e)
+      if (mask >> e & 1) {
+        if (at < kHold) {
+          hx[at] = v[e];
+          hi[at] = i + e;
+        }
+        ++at;
+      }
+    n += __shfl_sync(0xffffffffu, incl, 31);
+  });
+  __syncthreads();
+  if (lane == 0) sh.part[warp] = (uint64_t)n;
+  __syncthreads();
+  int here = 0, upto = 0;
+  bool fits = true;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int c = (int)sh.part[w];
+    fits = fits && c <= kHold;
+    if (w < warp) upto += c;
+    here += c;
+  }
+  // this warp's tokens, in registers while the list is filled
+  float kx[kHold / 32];
+  int ki[kHold / 32];
+#pragma unroll
+  for (int j = 0; j < kHold / 32; ++j) {
+    kx[j] = hx[j * 32 + lane];
+    ki[j] = hi[j * 32 + lane];
+  }
+  cl.gather(sh, 7, fits ? (uint64_t)here : (uint64_t)kList + 1);
+  int before = 0, total = 0;
+  for (int r = 0; r < cl.size; ++r) {
+    if (r < cl.rank) before += (int)sh.slot[7][r];
+    total += (int)sh.slot[7][r];
+  }
+  if (total > kList) return -1;
+  Shared* to = cl.of(&sh, 0);
+#pragma unroll
+  for (int j = 0; j < kHold / 32; ++j)
+    if (j * 32 + lane < n) {
+      to->list_x[before + upto + j * 32 + lane] = kx[j];
+      to->list_i[before + upto + j * 32 + lane] = ki[j];
+    }
+  cl.sync();
+  return total;
+}
+
+struct Filter {
+  int64_t k;
+  double p;
+  float least, u;
+  int V;
+};
+
+// Cuts and draws from `src`, whose tokens are in `in`; `q` is the selection that
+// has begun on the first of the two cuts that are on.  first: top index.
+template <typename S, typename W>
+__device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const Row& row,
+                             const Filter& f, uint32_t top_key, Search q, bool begun, W&& write) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Cut cut;
+  const Search fresh = {kLowest, top_key, 0, 0, q.round, false};
+  if (f.k > 0 && f.k < f.V) {
+    if (!begun) {
+      q = fresh;
+      q.need = (uint64_t)f.k;
+      narrow<false>(src, cl, sh, row, cut, q, true, 0.0);
+    }
+    begun = false;
+    if (!q.whole) cut = finish<false>(src, cl, sh, row, cut, q, 1);
+  }
+  if (f.p < 1.0) {
+    if (!begun) {
+      const int round = q.round;
+      q = fresh;
+      q.round = round;
+      narrow<true>(src, cl, sh, row, cut, q, true, f.p);
+    }
+    if (!q.whole) cut = finish<true>(src, cl, sh, row, cut, q, 3);
+  }
+  // min-p: the smallest logit whose weight is large enough, by 32-way search
+  if (f.least > 0.f) {
+    if (warp == 0) {
+      uint32_t lo = kLowest, hi = top_key;  // the answer lies in [lo, hi]: the largest qualifies
+      while (lo < hi) {
+        const uint32_t step = (hi - lo + 31) / 32;
+        const uint64_t k = (uint64_t)lo + (uint64_t)step * lane;
+        const bool ok = k >= hi || row.exact(value_of((uint32_t)k)) >= (double)f.least;
+        const unsigned m = __ballot_sync(0xffffffffu, ok);
+        const int j = m ? __ffs(m) - 1 : 32;
+        const uint64_t t = (uint64_t)lo + (uint64_t)step * j;
+        const uint32_t nh = t < hi ? (uint32_t)t : hi;
+        lo = j == 0 ? nh : (uint32_t)((uint64_t)lo + (uint64_t)step * (j - 1) + 1);
+        hi = nh;
+      }
+      if (lane == 0) sh.key[0] = lo;
+    }
+    __syncthreads();
+    const float x = value_of(sh.key[0]);
+    if (x > cut.x) {
+      cut.x = x;
+      cut.end = 0x7fffffff;
+    }
+  }
+  uint64_t large = 0, total;
+  const uint64_t small = each_weight(src, row, cut, sh.queue[warp],
+                                     [&](float, uint64_t w, bool valid) { large += valid ? w : 0; });
+  const uint64_t mine = warp_sum64(small + large);
+  auto value = [&](float x, int i) -> uint64_t { return cut.has(x, i) ? row.weight(x) : 0; };
+  const double u = f.u > 0.f ? (double)f.u : 0.0;
+  const int id = locate<true, true>(src, cl, sh, 5, u, mine, value, &total);
+  if (id >= 0 && threadIdx.x == 0) write(id, total);
+  if (u * (double)total >= (double)total) {
+    // u at or past 1 (or rounded to it): the last kept token
+    int last = -1;
+    each(src, [&](const float* x, int i) {
+#pragma unroll 1
+      for (int e = 0; e < S::N; ++e)
+        if (value(x[e], i + e) > 0) last = i + e;
+    });
+    last = __reduce_max_sync(0xffffffffu, last);
+    __syncthreads();
+    if (lane == 0) sh.part[warp] = (uint64_t)(int64_t)last;
+    __syncthreads();
+    for (int i = 0; i < kWarps; ++i) last = max(last, (int)(int64_t)sh.part[i]);
+    cl.gather(sh, 6, (uint64_t)(int64_t)last);
+    for (int i = 0; i < cl.size; ++i) last = max(last, (int)(int64_t)sh.slot[6][i]);
+    if (cl.rank == 0 && threadIdx.x == 0) write(last, total);
+  }
 }
 
 template <typename T>
@@ -419,20 +682,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   sl.base = v0 * Slice<T>::N - skew;
   sl.held = nullptr;
 
-  // hold it; the first token of the order: largest key, lowest index
-  uint64_t best = 0;
+  // hold it; the first token of the order: largest logit, lowest index (a lane's
+  // tokens ascend, so a larger one has to be larger)
+  float top = -INFINITY;
+  int first = 0;
 #pragma unroll 4
   for (int v = tid; v < sl.count; v += kThreads) {
     const Vec16<T> x = sl.fetch(v);
     if (a.resident) held[v] = *reinterpret_cast<const uint4*>(&x);
 #pragma unroll
     for (int e = 0; e < Slice<T>::N; ++e) {
-      const uint32_t i = (uint32_t)(sl.base + v * Slice<T>::N + e);
-      const uint64_t c = ((uint64_t)key_of(to_f32(x.v[e])) << 32) | ~i;
-      if (c > best) best = c;
+      const float f = to_f32(x.v[e]);
+      if (f > top) {
+        top = f;
+        first = sl.base + v * Slice<T>::N + e;
+      }
     }
   }
+  for (int i = tid; i < kTable; i += kThreads) sh.table[i] = exp2((double)i / kTable);
   if (a.resident) sl.held = held;
+  uint64_t best = ((uint64_t)key_of(top) << 32) | ~(uint32_t)first;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const uint64_t c = __shfl_xor_sync(0xffffffffu, best, o);
@@ -448,87 +717,62 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   for (int i = 0; i < cl.size; ++i)
     if (sh.slot[0][i] > best) best = sh.slot[0][i];
 
-  const float t = a.temperature ? a.temperature[r] : a.temperature_v;
-  const int64_t k = a.top_k ? a.top_k[r] : a.top_k_v;
+  float t = a.temperature ? a.temperature[r] : a.temperature_v;
+  if (t > 3.4028235e38f) t = 3.4028235e38f;
+  Filter f;
+  f.k = a.top_k ? a.top_k[r] : a.top_k_v;
   const float p = a.top_p ? a.top_p[r] : a.top_p_v;
-  const float least = a.min_p ? a.min_p[r] : a.min_p_v;
-  Row row;
-  row.top_key = (uint32_t)(best >> 32);
-  const int first = (int)~(uint32_t)best;
-  if (row.top_key == 0 || !(t > 0.f) || k == 1 || least > 1.f) {
+  f.p = p < 1.f ? (double)p : 1.0;  // NaN: off
+  f.least = a.min_p ? a.min_p[r] : a.min_p_v;
+  f.u = a.u[r];
+  f.V = a.V;
+  const uint32_t top_key = (uint32_t)(best >> 32);
+  if (top_key == 0 || !(t > 0.f) || f.k == 1 || f.least > 1.f) {
     if (cl.rank == 0 && tid == 0) {
-      a.id[r] = row.top_key == 0 ? -1 : first;
-      a.logprob[r] = row.top_key == 0 ? -INFINITY : 0.f;
+      a.id[r] = top_key == 0 ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
+      a.logprob[r] = top_key == 0 ? -INFINITY : 0.f;
     }
     cl.sync();  // no CTA leaves while another may still write to its slots
     return;
   }
-  row.top = value_of(row.top_key);
+  Row row;
+  row.top = value_of(top_key);
   row.inv_t = 1.0 / (double)t;
-  row.inv_t_f = (float)row.inv_t;
+  row.rate = row.inv_t * 1.4426950408889634;
+  row.rate_f = (float)row.rate;
+  row.table = sh.table;
 
-  Cut cut;
-  bool all = true;  // no cut yet
-  int round = 0;
-  if (k > 0 && k < a.V) {
-    cut = select<false>(sl, cl, sh, row, cut, all, (uint64_t)k, 0.0, 1, round);
-    all = false;
-  }
-  if (p < 1.f) {
-    cut = select<true>(sl, cl, sh, row, cut, all, 0, (double)p, 3, round);
-    all = false;
-  }
-  // min-p: the smallest key whose weight is large enough, by 32-way search
-  uint32_t least_key = 1;
-  if (least > 0.f) {
-    if (warp == 0) {
-      uint32_t lo = kLowest, hi = row.top_key;  // the answer lies in [lo, hi]: the largest qualifies
-      while (lo < hi) {
-        const uint32_t step = (hi - lo + 31) / 32;
-        const uint64_t q = (uint64_t)lo + (uint64_t)step * lane;
-        const bool ok = q >= hi || row.exact(value_of((uint32_t)q)) >= (double)least;
-        const unsigned m = __ballot_sync(0xffffffffu, ok);
-        const int f = m ? __ffs(m) - 1 : 32;
-        const uint64_t top = (uint64_t)lo + (uint64_t)step * f;
-        const uint32_t nh = top < hi ? (uint32_t)top : hi;
-        lo = f == 0 ? nh : (uint32_t)((uint64_t)lo + (uint64_t)step * (f - 1) + 1);
-        hi = nh;
-      }
-      if (lane == 0) sh.key[0] = lo;
-    }
-    __syncthreads();
-    least_key = sh.key[0];
-  }
-  auto kept = [&](float x, uint32_t key, int i) -> uint64_t {
-    return key >= least_key && (all || cut.has(key, i)) ? row.weight(x) : 0;
-  };
-  const float uf = a.u[r];
-  uint64_t total;
-  const int id = locate<true>(
-      sl, cl, sh, 5, uf > 0.f ? (double)uf : 0.0, kept, &total,
-      [](uint64_t sum, double u) { return u * (double)sum; });
-  auto write = [&](int i) {
+  auto write = [&](int i, uint64_t total) {
     const float x = to_f32(sl.row[i]);
     const double z = x == row.top ? 0.0 : ((double)x - (double)row.top) * row.inv_t;
     a.id[r] = i;
     a.logprob[r] = (float)(z - log((double)total / kOne));
   };
-  if (id >= 0 && tid == 0) write(id);
-  if (!(uf < 1.f) || (double)uf * (double)total >= (double)total) {
-    // u at or past 1 (or rounded to it): the last kept token
-    int last = -1;
-    sl.each([&](float x, uint32_t key, int i) {
-      if (key != 0 && kept(x, key, i) > 0) last = i;
-    });
-    last = __reduce_max_sync(0xffffffffu, last);
-    __syncthreads();
-    if (lane == 0) sh.part[warp] = (uint64_t)(int64_t)last;
-    __syncthreads();
-    for (int i = 0; i < kWarps; ++i) last = max(last, (int)(int64_t)sh.part[i]);
-    cl.gather(sh, 6, (uint64_t)(int64_t)last);
-    for (int i = 0; i < cl.size; ++i) last = max(last, (int)(int64_t)sh.slot[6][i]);
-    if (cl.rank == 0 && tid == 0) write(last);
+  // The first cut's first histogram; what lies from its bin up may fit the list.
+  Search q = {kLowest, top_key, 0, 0, 0, false};
+  const bool by_count = f.k > 0 && f.k < a.V, by_weight = f.p < 1.0;
+  bool begun = false;
+  if (cl.size > 1 && (by_count || by_weight)) {
+    Cut all;
+    begun = true;
+    if (by_count) {
+      q.need = (uint64_t)f.k;
+      narrow<false>(sl, cl, sh, row, all, q, true, 0.0);
+    } else {
+      narrow<true>(sl, cl, sh, row, all, q, true, f.p);
+    }
+    if (!q.whole) {
+      const int n = collect(sl, cl, sh, value_of(q.lo));
+      if (n >= 0) {
+        if (cl.rank == 0) {
+          const List list = {sh.list_x, sh.list_i, n};
+          cut_and_draw(list, Cluster{1, 0}, sh, row, f, top_key, q, begun, write);
+        }
+        return;  // nothing of the other CTAs is needed any more
+      }
+    }
   }
+  cut_and_draw(sl, cl, sh, row, f, top_key, q, begun, write);
   cl.sync();
 }
 
@@ -540,7 +784,7 @@ int launch(SampleArgs a, int64_t rows, cudaStream_t st) {
   const int64_t vectors = ((int64_t)a.V + 2 * N - 2) / N;  // whatever the rows' skew
   int size = 1;
   while (size < 8 && rows * size < 2 * num_sms() && (int64_t)a.V >= 4096 * size) size *= 2;
-  while (size < 8 && (vectors + size - 1) / size * 16 > 100 * 1024) size *= 2;
+  while (size < 8 && (vectors + size - 1) / size * 16 > 80 * 1024) size *= 2;
   while (size < kMaxCluster && (vectors + size - 1) / size * N > kMaxSlice) size *= 2;
   a.slice = (int)((vectors + size - 1) / size);
   a.resident = (size_t)a.slice * 16 <= kMaxResident;

@@ -15,9 +15,9 @@
 //
 // A choice at a border must not depend on the order of a sum, so weights are
 // summed as integers: W = round(2^43 w), which keeps V <= 2^20 of them below
-// 2^63 and is exact in any order.  Where w < 2^-24.5 it comes from the fp32
-// exponential (off by under 2^-18 of it, so by 2^-42 of the largest at most),
-// above from fp64: 2^(i/256) from a table times a quartic in the rest, |r| <=
+// 2^63 and is exact in any order.  Where w < 2^-18 it comes from the fp32
+// exponential, with what rounding took from its argument put back (off by
+// 2^-22 of it, so by 2^-40 of the largest at most), above from fp64: 2^(i/256) from a table times a quartic in the rest, |r| <=
 // 2^-9, good to 2^-50.
 //
 // A cluster of CTAs holds a row in shared memory, so HBM is read once; every
@@ -81,22 +81,32 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// What the weights and bins of a row are computed with.
+// What the weights and bins of a row are computed with.  LONG: x - top may be
+// rounded by enough to matter (fp32 logits; a 16-bit one has to be under 2^-13
+// of the top for any, and then that is under 2^-24 of the distance).
+template <bool LONG>
 struct Row {
   float top;
-  float rate_f;      // log2(e) / t
+  float rate_f, rate_lo;  // log2(e) / t, in two parts
   double inv_t, rate;
   const double* table;
 
   // log2 of the weight, in fp32: NaN at the top itself where the rate or the
   // top is infinite
   __device__ __forceinline__ float log2_weight(float x) const { return (x - top) * rate_f; }
-  __device__ __forceinline__ static bool small(float z) { return z < -24.5f; }
-  __device__ __forceinline__ static uint32_t small_weight(float z) {
-    // 2^43 2^z < 2^19, rounded by adding 2^23
+  __device__ __forceinline__ static bool small(float z) { return z < -18.f; }
+  __device__ __forceinline__ uint32_t small_weight(float x, float z) const {
     float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
-    return __float_as_uint(fmaf(w, (float)kOne, 8388608.f)) - 0x4b000000u;
+    w *= (float)kOne;
+    // x - top = d + e exactly; z + rest = (d + e) (rate_f + rate_lo)
+    const float d = x - top;
+    float rest = fmaf(d, rate_lo, fmaf(d, rate_f, -z));
+    if (LONG) {
+      const float b = d - x, e = (x - (d - b)) - (top + b);
+      rest = fmaf(e, rate_f, rest);
+    }
+    return __float2uint_rn(fmaf(w, 0.6931472f * rest, w));  // NaN (w = 0, z = -inf) is 0
   }
   __device__ __forceinline__ uint64_t large_weight(float x) const {
     if (x == top) return (uint64_t)kOne;
@@ -116,7 +126,7 @@ struct Row {
   }
   __device__ __forceinline__ uint64_t weight(float x) const {
     const float z = log2_weight(x);
-    return small(z) ? small_weight(z) : large_weight(x);
+    return small(z) ? small_weight(x, z) : large_weight(x);
   }
   __device__ __forceinline__ double exact(float x) const {
     return x == top ? 1.0 : exp(((double)x - (double)top) * inv_t);
@@ -135,7 +145,7 @@ struct Shared {
   uint32_t hist[2][3][kBins];      // 15-bit parts of the sums, two in turn
   uint64_t sums[kBins];            // over the cluster
   uint64_t slot[10][kMaxCluster];  // one exchange each
-  uint64_t part[kWarps];
+  uint64_t part[kWarps], walk[kWarps];
   uint64_t above;
   int bin, found;
   uint32_t key[2];
@@ -204,32 +214,38 @@ __device__ __forceinline__ void each(const S& src, F&& f) {
 
 // each() for weights: sink(x, W, valid) gets the large ones, a warp at a time;
 // the sum of this lane's small ones is returned.
-template <typename S, typename F>
-__device__ __forceinline__ uint64_t each_weight(const S& src, const Row& row, const Cut& cut,
+template <typename S, typename R, typename F>
+__device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, const Cut& cut,
                                                 float* queue, F&& sink) {
   const int lane = threadIdx.x & 31;
   const unsigned before = (1u << lane) - 1;
   uint64_t tail = 0;
   int waiting = 0, at = 0;
   each(src, [&](const float* x, int i) {
-    uint32_t small = 0;
+    uint32_t small = 0, large = 0;
 #pragma unroll
     for (int e = 0; e < S::N; ++e) {
       const float z = row.log2_weight(x[e]);
-      const bool in = cut.has(x[e], i + e), little = Row::small(z);
-      if (in && little) small += Row::small_weight(z);
-      const unsigned m = __ballot_sync(0xffffffffu, in && !little);
-      if (m) {
-        if (in && !little) queue[(at + waiting + __popc(m & before)) & 63] = x[e];
+      const bool in = cut.has(x[e], i + e), little = R::small(z);
+      const uint32_t w = row.small_weight(x[e], z);
+      small += in && little ? w : 0;
+      large |= in && !little ? 1u << e : 0;
+    }
+    if (__any_sync(0xffffffffu, large != 0)) {
+#pragma unroll
+      for (int e = 0; e < S::N; ++e) {
+        const bool mine = large >> e & 1;
+        const unsigned m = __ballot_sync(0xffffffffu, mine);
+        if (m == 0) continue;
+        if (mine) queue[(at + waiting + __popc(m & before)) & 63] = x[e];
         waiting += __popc(m);
-        if (waiting >= 32) {
-          __syncwarp();
-          const float q = queue[(at + lane) & 63];
-          __syncwarp();
-          at += 32;
-          waiting -= 32;
-          sink(q, row.large_weight(q), true);
-        }
+        if (waiting < 32) continue;
+        __syncwarp();
+        const float q = queue[(at + lane) & 63];
+        __syncwarp();
+        at += 32;
+        waiting -= 32;
+        sink(q, row.large_weight(q), true);
       }
     }
     tail += small;
@@ -306,12 +322,9 @@ __device__ int locate(const S& src, const Cluster& cl, Shared& sh, int step, dou
   if (lane == 0) sh.part[warp] = mine;
   if (threadIdx.x == 0) sh.found = -1;
   __syncthreads();
-  uint64_t here = 0, upto = 0;  // of the CTA, before this warp
+  uint64_t here = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += sh.part[w];
-    here += sh.part[w];
-  }
+  for (int w = 0; w < kWarps; ++w) here += sh.part[w];
   cl.gather(sh, step, here);
   uint64_t before = 0, total = 0;
   for (int r = 0; r < cl.size; ++r) {
@@ -321,40 +334,44 @@ __device__ int locate(const S& src, const Cluster& cl, Shared& sh, int step, dou
   *total_out = total;
   const double target = FRACTION ? want * (double)total : want;
   auto reached = [&](uint64_t s) { return OVER ? (double)s > target : (double)s >= target; };
-  uint64_t run = before + upto;
-  if (mine > 0 && !reached(run) && reached(run + mine)) {
-    // one warp of the cluster: walk its share
-    const int per = (src.count + kWarps - 1) / kWarps, end = min(src.count, (warp + 1) * per);
-    for (int v0 = warp * per; v0 < end; v0 += 32) {
-      const int v = v0 + lane;
-      float x[S::N];
-      uint64_t s = 0;
-      int i = 0;
-      if (v < end) {
-        src.get(v, x);
-        i = src.index(v);
-#pragma unroll 1
-        for (int e = 0; e < S::N; ++e) s += value(x[e], i + e);
-      }
-      const uint64_t incl = warp_scan64(s);
-      uint64_t at = run + incl - s;
-      const bool hit = s > 0 && !reached(at) && reached(at + s);
-      if (hit) {
-#pragma unroll 1
-        for (int e = 0; e < S::N; ++e) {
-          const uint64_t w = value(x[e], i + e);
-          if (w > 0 && reached(at + w)) {
-            sh.found = i + e;
-            break;
-          }
-          at += w;
-        }
-      }
-      if (__any_sync(0xffffffffu, hit)) break;
-      run += __shfl_sync(0xffffffffu, incl, 31);
+  if (reached(before) || !reached(before + here)) return -1;
+  // this CTA: the warp whose share it is, then a thread per vector of that share
+  uint64_t run = before;
+  int w = 0;
+  while (w < kWarps - 1 && !reached(run + sh.part[w])) run += sh.part[w++];
+  const int per = (src.count + kWarps - 1) / kWarps, end = min(src.count, (w + 1) * per);
+  for (int v0 = w * per; v0 < end; v0 += kThreads) {
+    const int v = v0 + threadIdx.x;
+    float x[S::N];
+    uint64_t s = 0;
+    int i = 0;
+    if (v < end) {
+      src.get(v, x);
+      i = src.index(v);
+#pragma unroll
+      for (int e = 0; e < S::N; ++e) s += value(x[e], i + e);
     }
+    uint64_t incl = warp_scan64(s), all = 0;
+    if (lane == 31) sh.walk[warp] = incl;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kWarps; ++j) {
+      if (j < warp) incl += sh.walk[j];
+      all += sh.walk[j];
+    }
+    uint64_t at = run + incl - s;
+    if (s > 0 && !reached(at) && reached(at + s)) {
+#pragma unroll
+      for (int e = 0; e < S::N; ++e) {
+        const uint64_t c = value(x[e], i + e);
+        if (c > 0 && !reached(at) && reached(at + c)) sh.found = i + e;
+        at += c;
+      }
+    }
+    run += all;
+    __syncthreads();
+    if (sh.found >= 0) break;
   }
-  __syncthreads();
   return sh.found;
 }
 
@@ -365,32 +382,42 @@ struct Search {
   uint64_t above, need;
   int round;    // histograms so far (of the two in turn)
   bool whole;   // nothing to cut
+  bool beyond;  // the last histogram's last bin
 };
 
-// One histogram of the tokens in `in` and [q.lo, q.hi], by distance to the top
-// (first = true) or by key; q narrows to the bin that the prefix ends in.
-// WEIGHT: q.need becomes p of the sum, on the first call with all tokens.
-template <bool WEIGHT, typename S>
-__device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const Row& row, const Cut& in,
-                       Search& q, bool first, double p) {
+// What a histogram's bins are: distances to the top, near or far, or keys.
+// Near: counts in bins of 1/16 over 32, weights in bins of 1/32 over 16 log2s;
+// far: twice as wide and long, from where the near ones end.
+enum Bins { kNear, kFar, kKeys };
+
+// One histogram of the tokens in `in` and [q.lo, q.hi]; q narrows to the bin
+// that the prefix ends in.  WEIGHT: q.need, where 0, becomes p of the sum.
+template <bool WEIGHT, Bins BINS, typename S, typename R>
+__device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row, const Cut& in,
+                       Search& q, double p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // counts: bins of 1/16 over 32; weights: of 1/32 over 16, in units of log2
-  const float per = WEIGHT ? row.rate_f * 32.f : 16.f;
-  auto distance = [&](float x) { return min(__float2int_rz((row.top - x) * per), kBins - 1); };
+  const float per = (WEIGHT ? row.rate_f * 32.f : 16.f) * (BINS == kFar ? 0.5f : 1.f);
+  auto distance = [&](float x) {
+    // (NaN, at the top where it or the rate is infinite, converts to 0)
+    const int d = __float2int_rz((row.top - x) * per) - (BINS == kFar ? kBins / 2 : 0);
+    return max(0, min(d, kBins - 1));
+  };
   const int bits = 32 - __clz(q.hi - q.lo);
   const int shift = bits > 9 ? bits - 9 : 0;
-  auto bin_of = [&](float x) { return first ? distance(x) : (int)((q.hi - key_of(x)) >> shift); };
+  auto bin_of = [&](float x) {
+    return BINS == kKeys ? (int)((q.hi - key_of(x)) >> shift) : distance(x);
+  };
   uint32_t (*hist)[kBins] = sh.hist[q.round & 1];
 #pragma unroll
   for (int i = 0; i < 3; ++i) hist[i][tid] = 0;
   __syncthreads();
   // keys and logits have the same order
   const float x_lo = value_of(q.lo), x_hi = value_of(q.hi);
-  if (WEIGHT && first) {
+  if (WEIGHT && BINS == kNear) {
     uint64_t tail = each_weight(src, row, in, sh.queue[warp], [&](float x, uint64_t w, bool valid) {
       add_warp(hist, distance(x), w, valid);
     });
-    tail = warp_sum64(tail);  // all of them lie in the last bin, or rate * 32 overflows
+    tail = warp_sum64(tail);  // small ones are past 18 log2s: all in the last bin
     if (lane == 0) add_parts(hist, kBins - 1, tail);
   } else {
     each(src, [&](const float* x, int i) {
@@ -424,7 +451,7 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const Row& r
     if (w < warp) incl += sh.part[w];
     total += sh.part[w];
   }
-  if (first) {
+  if (BINS == kNear) {
     if (WEIGHT && q.need == 0) {
       const double f = ceil(p * (double)total);
       q.need = f < 1.0 ? 1 : (uint64_t)f;
@@ -441,7 +468,8 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const Row& r
   __syncthreads();
   const int bin = sh.bin;
   q.above = sh.above;
-  if (!first) {
+  q.beyond = bin == kBins - 1;
+  if (BINS == kKeys) {
     const uint64_t down = (uint64_t)bin << shift;
     const uint32_t h = down <= q.hi - q.lo ? q.hi - (uint32_t)down : q.lo;
     const uint32_t span = (1u << shift) - 1;
@@ -476,11 +504,21 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const Row& r
   q.hi = sh.key[1] - 1;
 }
 
+// The histograms by distance; false where they go past the near ones.
+template <bool WEIGHT, typename S, typename R>
+__device__ bool begin(const S& src, const Cluster& cl, Shared& sh, const R& row, const Cut& in,
+                      Search& q, double p) {
+  narrow<WEIGHT, kNear>(src, cl, sh, row, in, q, p);
+  if (q.whole || !q.beyond) return true;
+  narrow<WEIGHT, kFar>(src, cl, sh, row, in, q, p);
+  return false;
+}
+
 // Narrows to one key and cuts the tokens equal to it by index.
-template <bool WEIGHT, typename S>
-__device__ Cut finish(const S& src, const Cluster& cl, Shared& sh, const Row& row, const Cut& in,
+template <bool WEIGHT, typename S, typename R>
+__device__ Cut finish(const S& src, const Cluster& cl, Shared& sh, const R& row, const Cut& in,
                       Search& q, int step) {
-  while (q.lo < q.hi) narrow<WEIGHT>(src, cl, sh, row, in, q, false, 0.0);
+  while (q.lo < q.hi) narrow<WEIGHT, kKeys>(src, cl, sh, row, in, q, 0.0);
   // as many as are still needed, lowest index first
   const float x = value_of(q.lo);
   const uint64_t each_w = WEIGHT ? row.weight(x) : 1;
@@ -584,17 +622,17 @@ struct Filter {
 
 // Cuts and draws from `src`, whose tokens are in `in`; `q` is the selection that
 // has begun on the first of the two cuts that are on.  first: top index.
-template <typename S, typename W>
-__device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const Row& row,
+template <typename S, typename R, typename W>
+__device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const R& row,
                              const Filter& f, uint32_t top_key, Search q, bool begun, W&& write) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Cut cut;
-  const Search fresh = {kLowest, top_key, 0, 0, q.round, false};
+  const Search fresh = {kLowest, top_key, 0, 0, q.round, false, false};
   if (f.k > 0 && f.k < f.V) {
     if (!begun) {
       q = fresh;
       q.need = (uint64_t)f.k;
-      narrow<false>(src, cl, sh, row, cut, q, true, 0.0);
+      begin<false>(src, cl, sh, row, cut, q, 0.0);
     }
     begun = false;
     if (!q.whole) cut = finish<false>(src, cl, sh, row, cut, q, 1);
@@ -604,7 +642,7 @@ __device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const 
       const int round = q.round;
       q = fresh;
       q.round = round;
-      narrow<true>(src, cl, sh, row, cut, q, true, f.p);
+      begin<true>(src, cl, sh, row, cut, q, f.p);
     }
     if (!q.whole) cut = finish<true>(src, cl, sh, row, cut, q, 3);
   }
@@ -640,6 +678,7 @@ __device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const 
   const double u = f.u > 0.f ? (double)f.u : 0.0;
   const int id = locate<true, true>(src, cl, sh, 5, u, mine, value, &total);
   if (id >= 0 && threadIdx.x == 0) write(id, total);
+  // (a CTA may leave from here on: what follows is for all or for none)
   if (u * (double)total >= (double)total) {
     // u at or past 1 (or rounded to it): the last kept token
     int last = -1;
@@ -682,40 +721,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   sl.base = v0 * Slice<T>::N - skew;
   sl.held = nullptr;
 
-  // hold it; the first token of the order: largest logit, lowest index (a lane's
-  // tokens ascend, so a larger one has to be larger)
+  // hold it, and find the largest logit
   float top = -INFINITY;
-  int first = 0;
 #pragma unroll 4
   for (int v = tid; v < sl.count; v += kThreads) {
     const Vec16<T> x = sl.fetch(v);
     if (a.resident) held[v] = *reinterpret_cast<const uint4*>(&x);
 #pragma unroll
-    for (int e = 0; e < Slice<T>::N; ++e) {
-      const float f = to_f32(x.v[e]);
-      if (f > top) {
-        top = f;
-        first = sl.base + v * Slice<T>::N + e;
-      }
-    }
+    for (int e = 0; e < Slice<T>::N; ++e) top = fmaxf(top, to_f32(x.v[e]));  // (not NaN)
   }
   for (int i = tid; i < kTable; i += kThreads) sh.table[i] = exp2((double)i / kTable);
   if (a.resident) sl.held = held;
-  uint64_t best = ((uint64_t)key_of(top) << 32) | ~(uint32_t)first;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t c = __shfl_xor_sync(0xffffffffu, best, o);
-    if (c > best) best = c;
-  }
-  if (lane == 0) sh.part[warp] = best;
+  const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of(top));
+  if (lane == 0) sh.part[warp] = mine;
   __syncthreads();
+  uint32_t top_key = 0;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i)
-    if (sh.part[i] > best) best = sh.part[i];
+  for (int i = 0; i < kWarps; ++i) top_key = max(top_key, (uint32_t)sh.part[i]);
   if (cl.size > 1) cg::this_cluster().barrier_wait();
-  cl.gather(sh, 0, best);
-  for (int i = 0; i < cl.size; ++i)
-    if (sh.slot[0][i] > best) best = sh.slot[0][i];
+  cl.gather(sh, 0, top_key);
+  for (int i = 0; i < cl.size; ++i) top_key = max(top_key, (uint32_t)sh.slot[0][i]);
 
   float t = a.temperature ? a.temperature[r] : a.temperature_v;
   if (t > 3.4028235e38f) t = 3.4028235e38f;
@@ -726,20 +751,34 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   f.least = a.min_p ? a.min_p[r] : a.min_p_v;
   f.u = a.u[r];
   f.V = a.V;
-  const uint32_t top_key = (uint32_t)(best >> 32);
   if (top_key == 0 || !(t > 0.f) || f.k == 1 || f.least > 1.f) {
+    // the first token of the order: the lowest index with the largest logit
+    int first = 0x7fffffff;
+    const float x_top = value_of(top_key);
+    each(sl, [&](const float* x, int i) {
+#pragma unroll
+      for (int e = 0; e < Slice<T>::N; ++e)
+        if (x[e] == x_top) first = min(first, i + e);
+    });
+    first = __reduce_min_sync(0xffffffffu, first);
+    __syncthreads();
+    if (lane == 0) sh.part[warp] = (uint64_t)first;
+    __syncthreads();
+    for (int i = 0; i < kWarps; ++i) first = min(first, (int)sh.part[i]);
+    cl.gather(sh, 1, (uint64_t)first);
+    for (int i = 0; i < cl.size; ++i) first = min(first, (int)sh.slot[1][i]);
     if (cl.rank == 0 && tid == 0) {
-      a.id[r] = top_key == 0 ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
+      a.id[r] = top_key == 0 ? -1 : (int64_t)first;
       a.logprob[r] = top_key == 0 ? -INFINITY : 0.f;
     }
-    cl.sync();  // no CTA leaves while another may still write to its slots
-    return;
+    return;  // every exchange is done
   }
-  Row row;
+  Row<sizeof(T) == 4> row;
   row.top = value_of(top_key);
   row.inv_t = 1.0 / (double)t;
   row.rate = row.inv_t * 1.4426950408889634;
   row.rate_f = (float)row.rate;
+  row.rate_lo = (float)(row.rate - (double)row.rate_f);
   row.table = sh.table;
 
   auto write = [&](int i, uint64_t total) {
@@ -749,19 +788,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     a.logprob[r] = (float)(z - log((double)total / kOne));
   };
   // The first cut's first histogram; what lies from its bin up may fit the list.
-  Search q = {kLowest, top_key, 0, 0, 0, false};
+  Search q = {kLowest, top_key, 0, 0, 0, false, false};
   const bool by_count = f.k > 0 && f.k < a.V, by_weight = f.p < 1.0;
   bool begun = false;
   if (cl.size > 1 && (by_count || by_weight)) {
     Cut all;
     begun = true;
+    bool near;  // far ones are many
     if (by_count) {
       q.need = (uint64_t)f.k;
-      narrow<false>(sl, cl, sh, row, all, q, true, 0.0);
+      near = begin<false>(sl, cl, sh, row, all, q, 0.0);
     } else {
-      narrow<true>(sl, cl, sh, row, all, q, true, f.p);
+      near = begin<true>(sl, cl, sh, row, all, q, f.p);
     }
-    if (!q.whole) {
+    if (!q.whole && near) {
       const int n = collect(sl, cl, sh, value_of(q.lo));
       if (n >= 0) {
         if (cl.rank == 0) {
@@ -773,7 +813,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
   }
   cut_and_draw(sl, cl, sh, row, f, top_key, q, begun, write);
-  cl.sync();
 }
 
 // CTAs per row: enough for two per SM, each with at least 2048 tokens, at most
@@ -783,7 +822,7 @@ int launch(SampleArgs a, int64_t rows, cudaStream_t st) {
   constexpr int N = 16 / (int)sizeof(T);
   const int64_t vectors = ((int64_t)a.V + 2 * N - 2) / N;  // whatever the rows' skew
   int size = 1;
-  while (size < 8 && rows * size < 2 * num_sms() && (int64_t)a.V >= 4096 * size) size *= 2;
+  while (size < 8 && rows * size < 4 * num_sms() && (int64_t)a.V >= 4096 * size) size *= 2;
   while (size < 8 && (vectors + size - 1) / size * 16 > 80 * 1024) size *= 2;
   while (size < kMaxCluster && (vectors + size - 1) / size * N > kMaxSlice) size *= 2;
   a.slice = (int)((vectors + size - 1) / size);

@@ -70,43 +70,73 @@ struct SampleArgs {
   float* logprob;
 };
 
-// Unsigned order of the key = order of the logits, masked ones 0.
+// Unsigned order of the key = order of the logits, masked ones 0.  The low G
+// bits of a widened 16-bit logit's key say nothing and are dropped.
+template <int G>
 __device__ __forceinline__ uint32_t key_of(float x) {
   if (!(x > -INFINITY)) return 0;  // NaN and -inf
   const uint32_t b = __float_as_uint(x + 0.f);  // -0 -> +0: equal logits, equal keys
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (b & 0x80000000u ? ~b : b | 0x80000000u) >> G;
 }
-constexpr uint32_t kLowest = 0x00800000u;  // of the lowest finite value
+template <int G>
 __device__ __forceinline__ float value_of(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+  key <<= G;
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key & (0xffffffffu << G));
 }
+template <int G>
+constexpr uint32_t kLowest = 0x00800000u >> G;  // of the lowest finite value, or just below
+template <typename T> constexpr int kDropped = 0;
+template <> constexpr int kDropped<__nv_bfloat16> = 16;
+template <> constexpr int kDropped<__half> = 13;
 
-// What the weights and bins of a row are computed with.  LONG: x - top may be
-// rounded by enough to matter (fp32 logits; a 16-bit one has to be under 2^-13
-// of the top for any, and then that is under 2^-24 of the distance).
-template <bool LONG>
+// What the weights and bins of a row are computed with; G: of its keys.
+//
+// log2 w = (x - shift) rate + c, shift = 0 and c = -top rate as a rule.  With rate
+// and c each in two parts, c_hi a multiple of 2^-11 under 2^12, the rest of it
+// after the nearest integer n is one fused multiply-add, (x - shift) rate_f +
+// (c_hi - n), whose addend is exact and whose result is under 1: off by 2^-25.
+// Where |top| rate passes 2^12, the tokens with any weight are within 1% of the
+// top: shift = top, x - top is exact and c = 0.
+template <int G>
 struct Row {
-  float top;
-  float rate_f, rate_lo;  // log2(e) / t, in two parts
+  static constexpr int kKey = G;
+  float top, shift;
+  float rate_f, rate_lo, c_hi, c_lo;
   double inv_t, rate;
   const double* table;
 
-  // log2 of the weight, in fp32: NaN at the top itself where the rate or the
-  // top is infinite
-  __device__ __forceinline__ float log2_weight(float x) const { return (x - top) * rate_f; }
+  // Returns false where only tokens equal to the top have weight (it is +inf,
+  // or the temperature so small that the next one below has none).
+  __device__ bool set(float top_, float t, const double* table_) {
+    top = top_;
+    table = table_;
+    inv_t = 1.0 / (double)t;
+    rate = inv_t * 1.4426950408889634;
+    const double c = -(double)top * rate;
+    shift = fabs(c) > 4096.0 ? top : 0.f;
+    c_hi = fabs(c) > 4096.0 ? 0.f : (float)(rint(c * 2048.0) * (1.0 / 2048.0));
+    c_lo = fabs(c) > 4096.0 ? 0.f : (float)(c - (double)c_hi);
+    rate_f = (float)rate;
+    rate_lo = (float)(rate - (double)rate_f);
+    if (top < INFINITY && fabs(c) < 4294967296.0 && rate < 1e30) return true;
+    shift = rate_f = rate_lo = c_hi = c_lo = 0.f;  // (unused: x == top comes first)
+    rate = 0.0;
+    return false;
+  }
+  __device__ __forceinline__ float log2_weight(float x) const {
+    return fmaf(x - shift, rate_f, c_hi);
+  }
   __device__ __forceinline__ static bool small(float z) { return z < -18.f; }
   __device__ __forceinline__ uint32_t small_weight(float x, float z) const {
+    const float d = x - shift;
+    const float shifted = fmaxf(z, -60.f) + 12582912.f;  // 1.5 * 2^23: its steps are 1
+    const float n = shifted - 12582912.f;
+    const float r = fmaf(d, rate_f, c_hi - n) + fmaf(d, rate_lo, c_lo);
     float w;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
-    w *= (float)kOne;
-    // x - top = d + e exactly; z + rest = (d + e) (rate_f + rate_lo)
-    const float d = x - top;
-    float rest = fmaf(d, rate_lo, fmaf(d, rate_f, -z));
-    if (LONG) {
-      const float b = d - x, e = (x - (d - b)) - (top + b);
-      rest = fmaf(e, rate_f, rest);
-    }
-    return __float2uint_rn(fmaf(w, 0.6931472f * rest, w));  // NaN (w = 0, z = -inf) is 0
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(r));
+    // times 2^(n + 43)
+    w = __uint_as_float(__float_as_uint(w) + (__float_as_uint(shifted) << 23) + (43u << 23));
+    return __float2uint_rn(w);
   }
   __device__ __forceinline__ uint64_t large_weight(float x) const {
     if (x == top) return (uint64_t)kOne;
@@ -136,7 +166,7 @@ struct Row {
 // Which tokens are left: logit > x, or equal and index < end.  (NaN never is.)
 struct Cut {
   float x = -INFINITY;
-  int end = 0;
+  int end = -0x7fffffff;  // below the negative indices of what lies before the row, too
   __device__ __forceinline__ bool has(float v, int i) const { return v > x || (v == x && i < end); }
 };
 
@@ -404,15 +434,10 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
   };
   const int bits = 32 - __clz(q.hi - q.lo);
   const int shift = bits > 9 ? bits - 9 : 0;
-  auto bin_of = [&](float x) {
-    return BINS == kKeys ? (int)((q.hi - key_of(x)) >> shift) : distance(x);
-  };
   uint32_t (*hist)[kBins] = sh.hist[q.round & 1];
 #pragma unroll
   for (int i = 0; i < 3; ++i) hist[i][tid] = 0;
   __syncthreads();
-  // keys and logits have the same order
-  const float x_lo = value_of(q.lo), x_hi = value_of(q.hi);
   if (WEIGHT && BINS == kNear) {
     uint64_t tail = each_weight(src, row, in, sh.queue[warp], [&](float x, uint64_t w, bool valid) {
       add_warp(hist, distance(x), w, valid);
@@ -422,11 +447,14 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
   } else {
     each(src, [&](const float* x, int i) {
 #pragma unroll
-      for (int e = 0; e < S::N; ++e)
-        if (x[e] >= x_lo && x[e] <= x_hi && in.has(x[e], i + e)) {
-          if (WEIGHT) add_parts(hist, bin_of(x[e]), row.weight(x[e]));
-          else atomicAdd(&hist[0][bin_of(x[e])], 1u);
-        }
+      for (int e = 0; e < S::N; ++e) {
+        // (by key: -0 has one of its own, which no token has)
+        const uint32_t key = key_of<R::kKey>(x[e]);
+        if (key < q.lo || key > q.hi || !in.has(x[e], i + e)) continue;
+        const int bin = BINS == kKeys ? (int)((q.hi - key) >> shift) : distance(x[e]);
+        if (WEIGHT) add_parts(hist, bin, row.weight(x[e]));
+        else atomicAdd(&hist[0][bin], 1u);
+      }
     });
   }
   cl.sync();
@@ -487,7 +515,7 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
       const uint64_t k = (uint64_t)a + (uint64_t)step * lane;
       bool ok = k >= b;
       if (!ok) {
-        const int d = distance(value_of((uint32_t)k));
+        const int d = distance(value_of<R::kKey>((uint32_t)k));
         ok = warp == 0 ? d <= bin : d < bin;
       }
       const unsigned m = __ballot_sync(0xffffffffu, ok);
@@ -520,7 +548,7 @@ __device__ Cut finish(const S& src, const Cluster& cl, Shared& sh, const R& row,
                       Search& q, int step) {
   while (q.lo < q.hi) narrow<WEIGHT, kKeys>(src, cl, sh, row, in, q, 0.0);
   // as many as are still needed, lowest index first
-  const float x = value_of(q.lo);
+  const float x = value_of<R::kKey>(q.lo);
   const uint64_t each_w = WEIGHT ? row.weight(x) : 1;
   const uint64_t want = (q.need - q.above + each_w - 1) / each_w;
   auto value = [&](float v, int i) -> uint64_t { return v == x && in.has(v, i); };
@@ -535,6 +563,7 @@ __device__ Cut finish(const S& src, const Cluster& cl, Shared& sh, const R& row,
   cl.gather(sh, step + 1, (uint64_t)(int64_t)at);
   Cut c;
   c.x = x;
+  c.end = 0;
   for (int r = 0; r < cl.size; ++r) c.end = max(c.end, (int)(int64_t)sh.slot[step + 1][r] + 1);
   return c;
 }
@@ -620,14 +649,86 @@ struct Filter {
   int V;
 };
 
+// Inclusive sums over the CTA, and the whole.
+__device__ __forceinline__ uint64_t block_scan(Shared& sh, uint64_t v, uint64_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_scan64(v);
+  __syncthreads();
+  if (lane == 31) sh.part[warp] = v;
+  __syncthreads();
+  uint64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) v += sh.part[w];
+    all += sh.part[w];
+  }
+  *total = all;
+  return v;
+}
+
+// The list's n <= kThreads tokens, a thread each: sorted, cut by rank and running
+// weight, put back in index order and drawn from.  need: the weight top-p asks
+// for, 0 where it is p of the first k.
+template <typename R, typename W>
+__device__ void draw_sorted(Shared& sh, const R& row, const Filter& f, int n, uint64_t need,
+                            W&& write) {
+  const int tid = threadIdx.x;
+  // largest first, then list (index) order; bitonic, by shuffles within a warp
+  uint64_t mine =
+      tid < n ? ((uint64_t)key_of<0>(sh.list_x[tid]) << 32) | ~(uint32_t)tid : (uint64_t)0;
+  int size = 32;
+  while (size < n) size *= 2;
+  for (int k = 2; k <= size; k *= 2) {
+    for (int j = k / 2; j > 0; j /= 2) {
+      uint64_t other;
+      if (j < 32) {
+        other = __shfl_xor_sync(0xffffffffu, mine, j);
+      } else {
+        __syncthreads();
+        sh.sums[tid] = mine;
+        __syncthreads();
+        other = sh.sums[tid ^ j];
+      }
+      const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
+      if ((mine < other) == larger) mine = other;
+    }
+  }
+  const bool on = mine != 0 && tid < n;
+  const int at = on ? (int)~(uint32_t)mine : 0;
+  __syncthreads();
+  sh.sums[tid] = 0;
+  const float x = on ? value_of<0>((uint32_t)(mine >> 32)) : row.top;
+  uint64_t w = on && (f.k <= 0 || tid < f.k) ? row.weight(x) : 0, total;
+  const uint64_t upto = block_scan(sh, w, &total);
+  if (f.p < 1.0) {
+    if (need == 0) {
+      const double c = ceil(f.p * (double)total);
+      need = c < 1.0 ? 1 : (uint64_t)c;
+    }
+    if (upto - w >= need) w = 0;
+  }
+  if (f.least > 0.f && tid > 0 && !(row.exact(x) >= (double)f.least)) w = 0;
+  if (on) sh.sums[at] = w;
+  __syncthreads();
+  w = sh.sums[tid];
+  const uint64_t run = block_scan(sh, w, &total);
+  if (tid == 0) sh.found = -1;
+  __syncthreads();
+  const double target = (f.u > 0.f ? (double)f.u : 0.0) * (double)total;
+  // (the last one where u is at or past 1, or rounded to it)
+  const bool end = target >= (double)total;
+  if (w > 0 && (end ? run == total : (double)run > target && !((double)(run - w) > target)))
+    write(sh.list_i[tid], total);
+}
+
 // Cuts and draws from `src`, whose tokens are in `in`; `q` is the selection that
 // has begun on the first of the two cuts that are on.  first: top index.
 template <typename S, typename R, typename W>
 __device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const R& row,
-                             const Filter& f, uint32_t top_key, Search q, bool begun, W&& write) {
+                             const Filter& f, Cut cut, uint32_t top_key, Search q, bool begun,
+                             W&& write) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Cut cut;
-  const Search fresh = {kLowest, top_key, 0, 0, q.round, false, false};
+  const Search fresh = {kLowest<R::kKey>, top_key, 0, 0, q.round, false, false};
   if (f.k > 0 && f.k < f.V) {
     if (!begun) {
       q = fresh;
@@ -649,11 +750,11 @@ __device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const 
   // min-p: the smallest logit whose weight is large enough, by 32-way search
   if (f.least > 0.f) {
     if (warp == 0) {
-      uint32_t lo = kLowest, hi = top_key;  // the answer lies in [lo, hi]: the largest qualifies
+      uint32_t lo = kLowest<R::kKey>, hi = top_key;  // the answer lies in [lo, hi]: the largest qualifies
       while (lo < hi) {
         const uint32_t step = (hi - lo + 31) / 32;
         const uint64_t k = (uint64_t)lo + (uint64_t)step * lane;
-        const bool ok = k >= hi || row.exact(value_of((uint32_t)k)) >= (double)f.least;
+        const bool ok = k >= hi || row.exact(value_of<R::kKey>((uint32_t)k)) >= (double)f.least;
         const unsigned m = __ballot_sync(0xffffffffu, ok);
         const int j = m ? __ffs(m) - 1 : 32;
         const uint64_t t = (uint64_t)lo + (uint64_t)step * j;
@@ -664,7 +765,7 @@ __device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const 
       if (lane == 0) sh.key[0] = lo;
     }
     __syncthreads();
-    const float x = value_of(sh.key[0]);
+    const float x = value_of<R::kKey>(sh.key[0]);
     if (x > cut.x) {
       cut.x = x;
       cut.end = 0x7fffffff;
@@ -706,6 +807,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   Cluster cl;
   cl.size = (int)cg::this_cluster().num_blocks();
   cl.rank = (int)cg::this_cluster().block_rank();
+  constexpr int G = kDropped<T>;
   const int64_t r = blockIdx.x / cl.size;
   // every CTA of the cluster has to run before another writes to its slots
   if (cl.size > 1) cg::this_cluster().barrier_arrive();
@@ -732,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
   for (int i = tid; i < kTable; i += kThreads) sh.table[i] = exp2((double)i / kTable);
   if (a.resident) sl.held = held;
-  const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of(top));
+  const uint32_t mine = __reduce_max_sync(0xffffffffu, key_of<G>(top));
   if (lane == 0) sh.part[warp] = mine;
   __syncthreads();
   uint32_t top_key = 0;
@@ -754,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (top_key == 0 || !(t > 0.f) || f.k == 1 || f.least > 1.f) {
     // the first token of the order: the lowest index with the largest logit
     int first = 0x7fffffff;
-    const float x_top = value_of(top_key);
+    const float x_top = top_key == 0 ? NAN : value_of<G>(top_key);
     each(sl, [&](const float* x, int i) {
 #pragma unroll
       for (int e = 0; e < Slice<T>::N; ++e)
@@ -773,13 +875,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     }
     return;  // every exchange is done
   }
-  Row<sizeof(T) == 4> row;
-  row.top = value_of(top_key);
-  row.inv_t = 1.0 / (double)t;
-  row.rate = row.inv_t * 1.4426950408889634;
-  row.rate_f = (float)row.rate;
-  row.rate_lo = (float)(row.rate - (double)row.rate_f);
-  row.table = sh.table;
+  Row<G> row;
+  Cut all;
+  if (!row.set(value_of<G>(top_key), t, sh.table)) {
+    all.x = row.top;
+    all.end = 0x7fffffff;
+  }
 
   auto write = [&](int i, uint64_t total) {
     const float x = to_f32(sl.row[i]);
@@ -788,11 +889,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     a.logprob[r] = (float)(z - log((double)total / kOne));
   };
   // The first cut's first histogram; what lies from its bin up may fit the list.
-  Search q = {kLowest, top_key, 0, 0, 0, false, false};
+  Search q = {kLowest<G>, top_key, 0, 0, 0, false, false};
   const bool by_count = f.k > 0 && f.k < a.V, by_weight = f.p < 1.0;
   bool begun = false;
-  if (cl.size > 1 && (by_count || by_weight)) {
-    Cut all;
+  if (by_count || by_weight) {
     begun = true;
     bool near;  // far ones are many
     if (by_count) {
@@ -802,17 +902,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       near = begin<true>(sl, cl, sh, row, all, q, f.p);
     }
     if (!q.whole && near) {
-      const int n = collect(sl, cl, sh, value_of(q.lo));
+      const int n = collect(sl, cl, sh, fmaxf(value_of<G>(q.lo), all.x));
       if (n >= 0) {
         if (cl.rank == 0) {
           const List list = {sh.list_x, sh.list_i, n};
-          cut_and_draw(list, Cluster{1, 0}, sh, row, f, top_key, q, begun, write);
+          if (n <= kThreads) draw_sorted(sh, row, f, n, by_count ? 0 : q.need, write);
+          else cut_and_draw(list, Cluster{1, 0}, sh, row, f, all, top_key, q, begun, write);
         }
         return;  // nothing of the other CTAs is needed any more
       }
     }
   }
-  cut_and_draw(sl, cl, sh, row, f, top_key, q, begun, write);
+  cut_and_draw(sl, cl, sh, row, f, all, top_key, q, begun, write);
 }
 
 // CTAs per row: enough for two per SM, each with at least 2048 tokens, at most

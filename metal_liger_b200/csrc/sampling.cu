@@ -100,13 +100,14 @@ template <> constexpr int kDropped<__half> = 13;
 template <int G>
 struct Row {
   static constexpr int kKey = G;
-  float top, shift;
+  float top, shift, floor;  // floor: its weight is 2^-60; nothing is smaller
   float rate_f, rate_lo, c_hi, c_lo;
   double inv_t, rate;
   const double* table;
 
-  // Returns false where only tokens equal to the top have weight (it is +inf,
-  // or the temperature so small that the next one below has none).
+  // Returns false where only tokens equal to the top have weight (it is +inf or
+  // the lowest of all, or the temperature so small that the next one below has
+  // none): the caller cuts the others.
   __device__ bool set(float top_, float t, const double* table_) {
     top = top_;
     table = table_;
@@ -118,24 +119,31 @@ struct Row {
     c_lo = fabs(c) > 4096.0 ? 0.f : (float)(c - (double)c_hi);
     rate_f = (float)rate;
     rate_lo = (float)(rate - (double)rate_f);
-    if (top < INFINITY && fabs(c) < 4294967296.0 && rate < 1e30) return true;
-    shift = rate_f = rate_lo = c_hi = c_lo = 0.f;  // (unused: x == top comes first)
-    rate = 0.0;
+    floor = fmaxf((float)((double)top - 60.0 / rate), -3.4028235e38f);
+    while (((double)top - (double)floor) * rate < 50.0 && top < INFINITY)  // rounded up
+      floor = value_of<0>(key_of<0>(floor) - 1);
+    if (top < INFINITY && floor > -INFINITY && fabs(c) < 4294967296.0 && rate < 1e30) return true;
+    // the top's log2 is 0 (or, of +inf, NaN: not small either)
+    const bool inf = !(top < INFINITY);
+    floor = -INFINITY;
+    shift = inf ? 0.f : top;
+    rate_f = inf ? 0.f : 1e30f;
+    c_hi = rate_lo = c_lo = 0.f;
     return false;
   }
   __device__ __forceinline__ float log2_weight(float x) const {
     return fmaf(x - shift, rate_f, c_hi);
   }
   __device__ __forceinline__ static bool small(float z) { return z < -18.f; }
+  // x >= floor.  43 is added to n on the way, for 2^43 w.
   __device__ __forceinline__ uint32_t small_weight(float x, float z) const {
     const float d = x - shift;
-    const float shifted = fmaxf(z, -60.f) + 12582912.f;  // 1.5 * 2^23: its steps are 1
-    const float n = shifted - 12582912.f;
+    const float shifted = z + 12582955.f;  // 1.5 * 2^23 + 43: its steps are 1
+    const float n = shifted - 12582955.f;
     const float r = fmaf(d, rate_f, c_hi - n) + fmaf(d, rate_lo, c_lo);
     float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(r));
-    // times 2^(n + 43)
-    w = __uint_as_float(__float_as_uint(w) + (__float_as_uint(shifted) << 23) + (43u << 23));
+    w = __uint_as_float(__float_as_uint(w) + (__float_as_uint(shifted) << 23));
     return __float2uint_rn(w);
   }
   __device__ __forceinline__ uint64_t large_weight(float x) const {
@@ -155,8 +163,8 @@ struct Row {
     return (uint64_t)__double_as_longlong(i) & 0xfffffffffffffull;
   }
   __device__ __forceinline__ uint64_t weight(float x) const {
-    const float z = log2_weight(x);
-    return small(z) ? small_weight(x, z) : large_weight(x);
+    const float y = fmaxf(x, floor), z = log2_weight(y);
+    return small(z) ? small_weight(y, z) : large_weight(x);
   }
   __device__ __forceinline__ double exact(float x) const {
     return x == top ? 1.0 : exp(((double)x - (double)top) * inv_t);
@@ -243,8 +251,8 @@ __device__ __forceinline__ void each(const S& src, F&& f) {
 }
 
 // each() for weights: sink(x, W, valid) gets the large ones, a warp at a time;
-// the sum of this lane's small ones is returned.
-template <typename S, typename R, typename F>
+// the sum of this lane's small ones is returned.  OPEN: the cut has everything.
+template <bool OPEN, typename S, typename R, typename F>
 __device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, const Cut& cut,
                                                 float* queue, F&& sink) {
   const int lane = threadIdx.x & 31;
@@ -255,11 +263,12 @@ __device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, cons
     uint32_t small = 0, large = 0;
 #pragma unroll
     for (int e = 0; e < S::N; ++e) {
-      const float z = row.log2_weight(x[e]);
-      const bool in = cut.has(x[e], i + e), little = R::small(z);
-      const uint32_t w = row.small_weight(x[e], z);
-      small += in && little ? w : 0;
-      large |= in && !little ? 1u << e : 0;
+      // (-inf and NaN take the floor's place, which weighs nothing)
+      const bool in = OPEN || cut.has(x[e], i + e);
+      const float y = fmaxf(x[e], row.floor), z = row.log2_weight(y);
+      const uint32_t w = row.small_weight(y, z);
+      if (!R::small(z)) large |= in ? 1u << e : 0;
+      else small += in ? w : 0;
     }
     if (__any_sync(0xffffffffu, large != 0)) {
 #pragma unroll
@@ -439,19 +448,22 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
   for (int i = 0; i < 3; ++i) hist[i][tid] = 0;
   __syncthreads();
   if (WEIGHT && BINS == kNear) {
-    uint64_t tail = each_weight(src, row, in, sh.queue[warp], [&](float x, uint64_t w, bool valid) {
+    uint64_t tail = each_weight<false>(src, row, in, sh.queue[warp], [&](float x, uint64_t w, bool valid) {
       add_warp(hist, distance(x), w, valid);
     });
     tail = warp_sum64(tail);  // small ones are past 18 log2s: all in the last bin
     if (lane == 0) add_parts(hist, kBins - 1, tail);
   } else {
+    // in the keys' range by value: -0 has a key of its own, which no token has
+    constexpr uint32_t kMinusZero = 0x7fffffffu >> R::kKey;
+    const float x_lo = value_of<R::kKey>(q.lo == kMinusZero ? q.lo + 1 : q.lo);
+    const float x_hi = value_of<R::kKey>(q.hi == kMinusZero ? q.hi - 1 : q.hi);
     each(src, [&](const float* x, int i) {
 #pragma unroll
       for (int e = 0; e < S::N; ++e) {
-        // (by key: -0 has one of its own, which no token has)
-        const uint32_t key = key_of<R::kKey>(x[e]);
-        if (key < q.lo || key > q.hi || !in.has(x[e], i + e)) continue;
-        const int bin = BINS == kKeys ? (int)((q.hi - key) >> shift) : distance(x[e]);
+        if (!(x[e] >= x_lo && x[e] <= x_hi) || !in.has(x[e], i + e)) continue;
+        const int bin =
+            BINS == kKeys ? (int)((q.hi - key_of<R::kKey>(x[e])) >> shift) : distance(x[e]);
         if (WEIGHT) add_parts(hist, bin, row.weight(x[e]));
         else atomicAdd(&hist[0][bin], 1u);
       }
@@ -772,8 +784,9 @@ __device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const 
     }
   }
   uint64_t large = 0, total;
-  const uint64_t small = each_weight(src, row, cut, sh.queue[warp],
-                                     [&](float, uint64_t w, bool valid) { large += valid ? w : 0; });
+  auto add = [&](float, uint64_t w, bool valid) { large += valid ? w : 0; };
+  const uint64_t small = cut.x == -INFINITY ? each_weight<true>(src, row, cut, sh.queue[warp], add)
+                                            : each_weight<false>(src, row, cut, sh.queue[warp], add);
   const uint64_t mine = warp_sum64(small + large);
   auto value = [&](float x, int i) -> uint64_t { return cut.has(x, i) ? row.weight(x) : 0; };
   const double u = f.u > 0.f ? (double)f.u : 0.0;
@@ -845,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   for (int i = 0; i < cl.size; ++i) top_key = max(top_key, (uint32_t)sh.slot[0][i]);
 
   float t = a.temperature ? a.temperature[r] : a.temperature_v;
-  if (t > 3.4028235e38f) t = 3.4028235e38f;
+  if (t > 1e30f) t = 1e30f;  // (all but uniform: floor stays finite)
   Filter f;
   f.k = a.top_k ? a.top_k[r] : a.top_k_v;
   const float p = a.top_p ? a.top_p[r] : a.top_p_v;

@@ -134,6 +134,24 @@ def test_parameters_per_row():
     _check(x, u, t, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_temperatures_and_logits_of_every_size(dtype):
+    """Weights from one token's to all equal, tops far from and at zero."""
+    gen = torch.Generator().manual_seed(10)
+    B, V = 5, 4099
+    for scale in (0.0, 1e-6, 1.0, 300.0, 6e4):
+        x = _logits(gen, B, V, torch.float32, scale)
+        x[1] -= 7.0
+        x[2] = -x[2].abs()                                       # the top at or next to zero
+        x[3] += torch.where(torch.arange(V) % 2 == 0, 0.0, -1.0) * scale
+        x = x.clamp(-6.5e4, 6.5e4).to(dtype)
+        u = torch.rand(B, generator=gen)
+        for t in (1e-38, 1e-30, 1e-9, 1e-4, 0.02, 30.0, 1e9, 1e35):
+            _check(x, u, t)
+            _check(x, u, t, top_p=0.7)
+            _check(x, u, t, top_k=100, top_p=0.9, min_p=0.3)
+
+
 def test_a_rows_token_does_not_depend_on_the_batch():
     gen = torch.Generator().manual_seed(7)
     x = _logits(gen, 200, 40000, torch.bfloat16, 1.0).to(DEV)

@@ -51,24 +51,43 @@ __device__ __forceinline__ float unpack(uint32_t w, int half) {
   return to_f32(v);
 }
 
-// Eight codes of a 16-byte vector; `mul` = qmax (times a power of two that
-// keeps x * qmax finite), `top` = a (times the same).
-template <typename T, int FMT>
-__device__ __forceinline__ uint2 quantise8(const uint4& x, float mul, float top) {
+// What a block's codes are computed with: x * mul / top, mul = qmax, both times
+// a power of two that keeps the product finite; inv = 1 / top, rounded.
+struct Divisor {
+  float mul, top, inv;
+};
+// p / top, correctly rounded: the product with the rounded reciprocal, corrected
+// by its remainder, which a fused multiply-add gives exactly (Markstein 1990).
+__device__ __forceinline__ float quotient(const Divisor& d, float x) {
+  const float p = x * d.mul, q = p * d.inv;
+  return fmaf(fmaf(-q, d.top, p), d.inv, q);
+}
+
+// Eight codes of a 16-byte vector.
+template <typename T, int FMT, bool TINY>
+__device__ __forceinline__ uint2 quantise8(const uint4& x, const Divisor& d) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t out[2] = {0, 0};
+  float q[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float a = __fdiv_rn(unpack<T>(w[i], 0) * mul, top);
-    const float b = __fdiv_rn(unpack<T>(w[i], 1) * mul, top);
-    uint32_t two;
+  for (int i = 0; i < 8; ++i) {
+    const float v = unpack<T>(w[i / 2], i & 1);
+    q[i] = TINY ? __fdiv_rn(v * d.mul, d.top) : quotient(d, v);
+  }
+  uint32_t out[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
     if (FMT == ML_KV8_INT8) {
-      two = (uint32_t)(uint8_t)(int8_t)__float2int_rn(a) |
-            ((uint32_t)(uint8_t)(int8_t)__float2int_rn(b) << 8);
+      uint32_t b[4];  // the code in the low byte: steps of 1 at 1.5 * 2^23
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(q[4 * i + j] + 12582912.f);
+      out[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     } else {
-      two = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]),
+                                                   __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[4 * i + 2], q[4 * i + 3]),
+                                                   __NV_SATFINITE, __NV_E4M3);
+      out[i] = lo | (hi << 16);
     }
-    out[i >> 1] |= two << (16 * (i & 1));
   }
   return make_uint2(out[0], out[1]);
 }
@@ -83,8 +102,12 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, int which, int
   const int64_t base = blk * a.block;
   const int live = (int)min((int64_t)a.block, end - base);
   const int64_t bh = (int64_t)b * a.heads + h;
+  // row 0 of the block, in the call's rows (that far before them, where start
+  // lies inside the block)
+  const int64_t pitch = a.stride[which][2];
   const T* src = static_cast<const T*>(a.src[which]) + b * a.stride[which][0] +
-                 h * a.stride[which][1];
+                 h * a.stride[which][1] + (base - start) * pitch;
+  const int fresh = (int)(start > base ? start - base : 0);  // first new row
   T* tail = static_cast<T*>(a.tail[which]) + (bh * 2 + (blk & 1)) * a.block * D;
   uint4 x[NV];
   uint32_t top2 = 0;  // |bits| maxima of even and odd elements
@@ -94,8 +117,7 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, int which, int
     const int row = v / VPR, col = (v % VPR) * 8;
     x[i] = make_uint4(0, 0, 0, 0);
     if (row < live) {
-      const int64_t p = base + row;
-      const T* from = p < start ? tail + row * D + col : src + (p - start) * a.stride[which][2] + col;
+      const T* from = row < fresh ? tail + row * D + col : src + row * pitch + col;
       x[i] = *reinterpret_cast<const uint4*>(from);
     }
     top2 = __vmaxu2(top2, x[i].x & 0x7fff7fffu);
@@ -117,30 +139,43 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, int which, int
   // x * qmax has to stay finite: values near the top of bf16 are halved 16
   // times on both sides of the division first (exact)
   const float down = amax > 1e30f ? 1.52587890625e-5f : 1.f;
+  Divisor d;
+  d.mul = qmax * down;
+  d.top = amax * down;
+  d.inv = __frcp_rn(d.top);
   uint8_t* codes = a.codes[which] + (bh * a.max_len + base) * D;
+  auto store = [&](auto&& quantise) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = i * kThreads + threadIdx.x;
-    const int row = v / VPR, col = (v % VPR) * 8;
-    if (row >= live) continue;
-    uint2 q = make_uint2(0, 0);
-    if (finite) q = quantise8<T, FMT>(x[i], qmax * down, amax * down);
-    *reinterpret_cast<uint2*>(codes + (int64_t)row * D + col) = q;
-    if (keep && base + row >= start) *reinterpret_cast<uint4*>(tail + row * D + col) = x[i];
-  }
+    for (int i = 0; i < NV; ++i) {
+      const int v = i * kThreads + threadIdx.x;
+      const int row = v / VPR, col = (v % VPR) * 8;
+      if (row >= live) continue;
+      *reinterpret_cast<uint2*>(codes + row * D + col) = quantise(x[i]);
+      if (keep && row >= fresh) *reinterpret_cast<uint4*>(tail + row * D + col) = x[i];
+    }
+  };
+  if (!finite)
+    store([](const uint4&) { return make_uint2(0, 0); });
+  else if (d.top < 1e-20f)  // so small that remainders would be rounded
+    store([&](const uint4& y) { return quantise8<T, FMT, true>(y, d); });
+  else
+    store([&](const uint4& y) { return quantise8<T, FMT, false>(y, d); });
 }
 
-// Grid (blocks a call can touch, kv heads x {K, V}, batch).
+// Grid ({K, V} x kv heads, blocks a call can touch, batch): heads next to one
+// another, as the projections leave them in a token's row.
 template <typename T, int FMT, int D, int NV>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, NV <= 4 ? 6 : NV == 8 ? 4 : 2)
 kv8_append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ uint32_t red[kThreads / 32];
-  const int b = blockIdx.z, which = blockIdx.y & 1, h = blockIdx.y >> 1;
+  pdl_wait();
+  pdl_release();
+  const int b = blockIdx.z, h = blockIdx.x >> 1, which = blockIdx.x & 1;
   const int64_t start = a.span.first(b);
   if (start < 0 || start >= a.max_len) return;
   const int64_t end = min((int64_t)a.max_len, start + a.span.count(b));
   const int64_t first = start / a.block, last = (end - 1) / a.block;
-  const int64_t blk = first + blockIdx.x;
+  const int64_t blk = first + blockIdx.y;
   if (end <= start || blk > last) return;
   // The block that replaces the tail slot the first block still reads (the
   // last or the one before, of the first one's parity) is done by the same
@@ -159,13 +194,14 @@ template <typename T, int FMT, int D>
 int launch_append(const AppendArgs& a, dim3 grid, cudaStream_t st) {
   switch (a.block * (D / 8) / kThreads) {
 #define ML_KV8_NV(NV_) \
-  case NV_: kv8_append_kernel<T, FMT, D, NV_><<<grid, kThreads, 0, st>>>(a); break;
+  case NV_:                                                                               \
+    ML_CHECK_CUDA(launch_pdl(kv8_append_kernel<T, FMT, D, NV_>, grid, dim3(kThreads), 0, st, a), \
+                  "kv8_append");                                                          \
+    return ML_OK;
     ML_KV8_NV(1) ML_KV8_NV(2) ML_KV8_NV(4) ML_KV8_NV(8) ML_KV8_NV(16)
 #undef ML_KV8_NV
     default: set_error("kv8_append: unsupported block size"); return ML_ERR_INVALID_ARG;
   }
-  ML_CHECK_LAUNCH("kv8_append");
-  return ML_OK;
 }
 
 template <typename T, int FMT>
@@ -218,7 +254,8 @@ extern "C" int ml_kv8_append(const ml_kv8_cache* cache, const void* k, const int
   // an unaligned start can touch one block more than the rows fill
   const int64_t nblk = (tokens + cache->block - 2) / cache->block + 1;
   const int64_t most = cache->max_len / cache->block;
-  const dim3 grid((unsigned)(nblk < most ? nblk : most), (unsigned)(2 * cache->kv_heads),
+  ML_CHECK_ARG(most <= 65535 || nblk <= 65535, "kv8_append: too many blocks in one call");
+  const dim3 grid((unsigned)(2 * cache->kv_heads), (unsigned)(nblk < most ? nblk : most),
                   (unsigned)cache->batch);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf = cache->dtype == ML_DTYPE_BF16;

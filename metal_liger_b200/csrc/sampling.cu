@@ -49,10 +49,12 @@ constexpr int kMaxCluster = 16;
 constexpr int kMaxSlice = 65536;     // tokens of a CTA: the histogram's 32-bit parts hold them
 constexpr int64_t kMaxVocab = (int64_t)1 << 20;
 constexpr double kOne = 8796093022208.0;  // 2^43
-constexpr size_t kMaxResident = 160 * 1024;
+// A slice that leaves room for two CTAs on an SM is held; a larger one is read
+// again from L2 (256 fp32 rows: 107 us, against 145 held by one CTA per SM).
+constexpr size_t kMaxResident = 80 * 1024;
 constexpr int kList = 1024;          // tokens of the list
 constexpr int kWarpList = kList / kWarps;  // of them from one warp
-constexpr int kTable = 256;
+constexpr int kTable = 64;
 
 struct SampleArgs {
   const void* logits;  // [rows, V] at row pitch ld
@@ -149,16 +151,17 @@ struct Row {
   __device__ __forceinline__ uint64_t large_weight(float x) const {
     if (x == top) return (uint64_t)kOne;
     const double y = ((double)x - (double)top) * rate;
-    const double magic = 26388279066624.0;  // 1.5 * 2^44: its steps are 2^-8
+    const double magic = 105553116266496.0;  // 1.5 * 2^46: its steps are 2^-6
     const double shifted = y + magic;
     const int k = __double2loint(shifted);
     const double r = y - (shifted - magic);
     // 2^r - 1
-    const double p = r * fma(r, fma(r, fma(r, 0.009618129107628477, 0.05550410866482158),
-                                    0.24022650695910072), 0.6931471805599453);
+    const double p = r * fma(r, fma(r, fma(r, fma(r, 0.0013333558146428443, 0.009618129107628477),
+                                           0.05550410866482158), 0.24022650695910072),
+                             0.6931471805599453);
     const double t = table[k & (kTable - 1)];
     double w = fma(t, p, t);
-    w = __hiloint2double(__double2hiint(w) + ((k >> 8) << 20), __double2loint(w));
+    w = __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
     const double i = fma(w, kOne, 4503599627370496.0);  // + 2^52: the integer in its low bits
     return (uint64_t)__double_as_longlong(i) & 0xfffffffffffffull;
   }
@@ -929,15 +932,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   cut_and_draw(sl, cl, sh, row, f, all, top_key, q, begun, write);
 }
 
-// CTAs per row: enough for two per SM, each with at least 2048 tokens, at most
-// kMaxSlice, and 16-byte vectors that fit shared memory twice per SM.
+// CTAs per row.  Few rows: eight, so that a row's passes are short (clusters of
+// eight are placed within a GPC, so more than 32 rows of them would queue).
+// More rows: four; with 256 rows of 151936 logits, four take 98 us (bf16, all
+// tokens open) and 271 us (top-p 0.95), eight 121 and 314 us, one 114 and 481
+// us.  At least 2048 tokens to a CTA, at most kMaxSlice.
 template <typename T>
 int launch(SampleArgs a, int64_t rows, cudaStream_t st) {
   constexpr int N = 16 / (int)sizeof(T);
   const int64_t vectors = ((int64_t)a.V + 2 * N - 2) / N;  // whatever the rows' skew
+  const int most = rows <= 32 ? 8 : 4;
   int size = 1;
-  while (size < 8 && rows * size < 4 * num_sms() && (int64_t)a.V >= 4096 * size) size *= 2;
-  while (size < 8 && (vectors + size - 1) / size * 16 > 80 * 1024) size *= 2;
+  while (size < most && (int64_t)a.V >= 4096 * size) size *= 2;
   while (size < kMaxCluster && (vectors + size - 1) / size * N > kMaxSlice) size *= 2;
   a.slice = (int)((vectors + size - 1) / size);
   a.resident = (size_t)a.slice * 16 <= kMaxResident;

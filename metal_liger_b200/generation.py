@@ -25,7 +25,13 @@ On B200:
 * for Qwen3-VL text prompts the decoder gets explicit [3, B, q] positions,
   which skips its per-forward device-to-host sync;
 * the sampling step takes its logits from this library's GEMM (bf16, the
-  logit dtype of a bf16 model) and samples with torch;
+  logit dtype of a bf16 model) and samples with torch, or, with
+  ``fused_sampling`` (or ``top_k`` / ``min_p``, which the reference lacks),
+  with this library's sampler, which honours ``top_p`` and runs inside the
+  captured decode step;
+* with ``kv_cache_dtype`` "int8" or "fp8" the cache is held in 8 bits
+  (``MetalLigerQuantizedCache``): half the memory per position, and half the
+  bytes a decode step reads;
 * generated ids go into one preallocated [batch, prompt + max_new_tokens]
   device buffer instead of a ``torch.cat`` per token.
 
@@ -99,6 +105,14 @@ class MetalLigerStaticCache(Cache):
     generation.py:18-66)."""
 
     def __init__(self, model: nn.Module, batch_size: int, max_seq_len: int):
+        self._describe(model, batch_size, max_seq_len)
+        shape = (self.num_layers, self.batch_size, self.num_kv_heads, self.max_seq_len,
+                 self.head_dim)
+        self.key_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
+        self.value_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
+        super().__init__(layers=[_StaticKVLayer(self, i) for i in range(self.num_layers)])
+
+    def _describe(self, model: nn.Module, batch_size: int, max_seq_len: int) -> None:
         p = next(model.parameters())
         self.device = p.device
         self.dtype = p.dtype
@@ -110,15 +124,10 @@ class MetalLigerStaticCache(Cache):
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.num_heads
         self.batch_size = int(batch_size)
         self.max_seq_len = int(max_seq_len)
-        shape = (self.num_layers, self.batch_size, self.num_kv_heads, self.max_seq_len,
-                 self.head_dim)
-        self.key_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
-        self.value_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
         self.seen_tokens = 0
         # Set while decoding on a CUDA graph: the int64 [1] device tensor
         # holding the position being written (see MetalLigerGenerator).
         self.graph_pos: Optional[Tensor] = None
-        super().__init__(layers=[_StaticKVLayer(self, i) for i in range(self.num_layers)])
 
     def update(self, key_states: Tensor, value_states: Tensor, layer_idx: int,
                cache_kwargs=None):
@@ -152,6 +161,144 @@ class MetalLigerStaticCache(Cache):
 
     def get_max_cache_shape(self, layer_idx: int = 0) -> int:
         return self.max_seq_len
+
+
+class MetalLigerQuantizedCache(MetalLigerStaticCache):
+    """The static cache held in 8 bits (``ops.quantized_kv``): int8 or e4m3
+    codes with a scale per block of positions and kv head.  The prompt's own
+    attention uses its keys and values as they are; decode steps attend to the
+    codes.  No counterpart in the reference."""
+
+    def __init__(self, model: nn.Module, batch_size: int, max_seq_len: int,
+                 cache_dtype: str = "int8", block: int = 64):
+        from metal_liger_b200.ops.quantized_kv import allocate_quantized_kv
+
+        p = next(model.parameters())
+        self._describe(model, batch_size, max_seq_len)
+        self.cache_dtype = cache_dtype
+        self.kv = [allocate_quantized_kv(self.batch_size, self.num_kv_heads, self.max_seq_len,
+                                         self.head_dim, cache_dtype, p.dtype, block, p.device)
+                   for _ in range(self.num_layers)]
+        self.start = torch.zeros(1, dtype=torch.int64, device=p.device)
+        # Rows given to a layer's update() that its attention has yet to ask
+        # for (see _QuantizedAttention).
+        self.pending: Optional[set] = None
+        self._rows = None
+        Cache.__init__(self, layers=[_QuantizedKVLayer(self, i) for i in range(self.num_layers)])
+
+    def _positions(self) -> Tensor:
+        """Device tensor of the number of positions filled before this step."""
+        if self.graph_pos is not None:
+            return self.graph_pos
+        return self.start.fill_(self.seen_tokens)
+
+    def update(self, key_states: Tensor, value_states: Tensor, layer_idx: int,
+               cache_kwargs=None):
+        """Append the new positions of layer ``layer_idx``.  Returns the prompt's
+        own keys / values on the first call and, outside ``_QuantizedAttention``,
+        the dequantised ones up to the current length; inside it, what is
+        returned is not used (the attention reads the codes)."""
+        from metal_liger_b200.ops.quantized_kv import quantized_kv_append
+
+        if self.graph_pos is None:
+            end = self.seen_tokens + key_states.shape[-2]
+            if end > self.max_seq_len:
+                raise RuntimeError(f"MetalLigerQuantizedCache: {end} positions exceed max_seq_len "
+                                   f"{self.max_seq_len}")
+        quantized_kv_append(self.kv[layer_idx], key_states, value_states, self._positions())
+        if self.pending is not None:
+            self.pending.add(layer_idx)
+            return key_states, value_states
+        if self.graph_pos is None and self.seen_tokens == 0:
+            return key_states, value_states
+        k, v = self.kv[layer_idx].dequantize()
+        if self.graph_pos is not None:
+            return k, v
+        return k[:, :, :end], v[:, :, :end]
+
+    def step_rows(self, pos: Tensor):
+        """(K, V, position 0): a cache of one position, where the fused q/k
+        norm + RoPE kernel leaves a step's rows for the append.  Layers share
+        it (they follow one another); it lives as long as this cache, which
+        the captured step's owner keeps."""
+        if self._rows is None:
+            shape = (self.batch_size, self.num_kv_heads, 1, self.head_dim)
+            self._rows = (torch.empty(shape, dtype=self.dtype, device=pos.device),
+                          torch.empty(shape, dtype=self.dtype, device=pos.device),
+                          torch.zeros_like(pos))
+        return self._rows
+
+    def decode_attention(self, layer_idx: int, query: Tensor, scale: float) -> Tensor:
+        """Attention of the step's query tokens [B, Hq, T, D], after their
+        keys and values were appended; [B, T, Hq, D]."""
+        from metal_liger_b200.ops.quantized_kv import quantized_kv_attention
+
+        return quantized_kv_attention(query, self.kv[layer_idx], self._positions(), scale=scale)
+
+
+class _QuantizedKVLayer(_StaticKVLayer):
+    def __init__(self, owner: MetalLigerQuantizedCache, idx: int):
+        CacheLayerMixin.__init__(self)
+        self.owner = owner
+        self.idx = idx
+        self.keys = owner.kv[idx].k_codes
+        self.values = owner.kv[idx].v_codes
+        self.is_initialized = True
+        self.max_batch_size = owner.batch_size
+        self.max_cache_len = owner.max_seq_len
+
+
+_KV8_ATTN = "metal_liger_kv8"
+_KV8_CACHE: list = [None]
+
+
+def _kv8_attention_forward(module, query, key, value, attention_mask, dropout=0.0, scaling=None,
+                           **kwargs):
+    from transformers.integrations.sdpa_attention import sdpa_attention_forward
+
+    cache = _KV8_CACHE[0]
+    layer = getattr(module, "layer_idx", None)
+    if cache is None or cache.pending is None or layer not in cache.pending:
+        return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
+                                      scaling=scaling, **kwargs)
+    cache.pending.discard(layer)
+    scale = float(scaling) if scaling is not None else query.shape[-1] ** -0.5
+    return cache.decode_attention(layer, query, scale), None
+
+
+class _QuantizedAttention:
+    """While a step decodes over a ``MetalLigerQuantizedCache``: the decoder's
+    attention reads the codes.  A decoder whose layers do not go through
+    transformers' attention interface is refused (its update()s would be
+    left unanswered)."""
+
+    def __init__(self, module: nn.Module, cache: MetalLigerStaticCache):
+        self.config = getattr(module, "config", None)
+        self.cache = cache if isinstance(cache, MetalLigerQuantizedCache) else None
+
+    def __enter__(self):
+        if self.cache is None:
+            return self
+        self.attn_prev = getattr(self.config, "_attn_implementation", None)
+        self.cache_prev = _KV8_CACHE[0]
+        if self.attn_prev is None:
+            raise RuntimeError("kv_cache_dtype: the decoder has no attention implementation to "
+                               "replace (config._attn_implementation)")
+        self.config._attn_implementation = _KV8_ATTN
+        _KV8_CACHE[0] = self.cache
+        self.cache.pending = set()
+        return self
+
+    def __exit__(self, exc_type, *exc):
+        if self.cache is None:
+            return False
+        left, self.cache.pending = self.cache.pending, None
+        self.config._attn_implementation = self.attn_prev
+        _KV8_CACHE[0] = self.cache_prev
+        if left and exc_type is None:
+            raise RuntimeError(f"kv_cache_dtype: layers {sorted(left)} did not attend through "
+                               "transformers' attention interface")
+        return False
 
 
 # Decode-step attention: registered with transformers' attention interface
@@ -188,6 +335,7 @@ def _register_decode_attention() -> bool:
     except ImportError:  # pragma: no cover - transformers is part of the image
         return False
     AttentionInterface.register(_DECODE_ATTN, _decode_attention_forward)
+    AttentionInterface.register(_KV8_ATTN, _kv8_attention_forward)
     return True
 
 
@@ -219,7 +367,8 @@ class _DecodeKernels:
         from metal_liger_b200 import _torch_library  # noqa: F401  (registers the ops)
 
         cfg = getattr(self.module, "config", None)
-        if self.pos is not None and cfg is not None and \
+        quantized = isinstance(self.cache, MetalLigerQuantizedCache)
+        if self.pos is not None and cfg is not None and not quantized and \
                 getattr(cfg, "_attn_implementation", None) == "sdpa":
             self.attn_prev = cfg._attn_implementation
             cfg._attn_implementation = _DECODE_ATTN
@@ -315,10 +464,8 @@ def _decode_block_ok(attn, cache) -> bool:
 
 def _decode_block_forward(attn, cache, pos: Tensor):
     orig = type(attn).forward
-    layer = attn.layer_idx
-    D = attn.head_dim
     projs = [attn.q_proj, attn.k_proj, attn.v_proj]
-    kc, vc = cache.key_cache[layer], cache.value_cache[layer]
+    attend = _decode_attend(attn, cache, pos)
 
     def forward(hidden_states, position_embeddings=None, attention_mask=None,
                 past_key_values=None, **kwargs):
@@ -329,14 +476,45 @@ def _decode_block_forward(attn, cache, pos: Tensor):
                         past_key_values, **kwargs)
         ops = torch.ops.metal_liger
         q, k, v = ops.gemv_multi(hidden_states, [p.weight for p in projs], [p.bias for p in projs])
-        cos, sin = position_embeddings
-        q4 = ops.decode_qk_norm_rope(q, k, v, attn.q_norm.weight, attn.k_norm.weight,
-                                     float(attn.q_norm.eps), float(attn.k_norm.eps), cos, sin,
-                                     kc, vc, pos)
-        out = ops.decode_attention(q4, kc, vc, pos, 1, float(attn.scaling))
+        out = attend(q, k, v, *position_embeddings)
         return attn.o_proj(out.reshape(B, S, -1)), None
 
     return forward
+
+
+def _decode_attend(attn, cache, pos: Tensor, one_launch: bool = False):
+    """The attention block's step between its projections: per-head norms and
+    RoPE of q and k, the cache write and the attention, [B, 1, Hq, D].
+    ``one_launch``: in a single launch where the cache is short enough."""
+    layer = attn.layer_idx
+    ops = torch.ops.metal_liger
+    if isinstance(cache, MetalLigerQuantizedCache):
+        from metal_liger_b200.ops.quantized_kv import quantized_kv_append
+
+        kv = cache.kv[layer]
+        k_row, v_row, first = cache.step_rows(pos)
+
+        def attend(q, k, v, cos, sin):
+            q4 = ops.decode_qk_norm_rope(q, k, v, attn.q_norm.weight, attn.k_norm.weight,
+                                         float(attn.q_norm.eps), float(attn.k_norm.eps), cos, sin,
+                                         k_row, v_row, first)
+            quantized_kv_append(kv, k_row, v_row, pos)
+            return cache.decode_attention(layer, q4, float(attn.scaling))
+
+        return attend
+    kc, vc = cache.key_cache[layer], cache.value_cache[layer]
+
+    def attend(q, k, v, cos, sin):
+        if one_launch and kc.shape[2] <= 256:  # q/k prep and attention in one launch
+            return ops.decode_qk_attention(q, k, v, attn.q_norm.weight, attn.k_norm.weight,
+                                           float(attn.q_norm.eps), float(attn.k_norm.eps), cos,
+                                           sin, kc, vc, pos, float(attn.scaling))
+        q4 = ops.decode_qk_norm_rope(q, k, v, attn.q_norm.weight, attn.k_norm.weight,
+                                     float(attn.q_norm.eps), float(attn.k_norm.eps), cos, sin,
+                                     kc, vc, pos)
+        return ops.decode_attention(q4, kc, vc, pos, 1, float(attn.scaling))
+
+    return attend
 
 
 # Decoder layers whose forward is, for one decode token, exactly: residual =
@@ -381,7 +559,7 @@ def _decode_layer_forward(layer, cache, pos: Tensor):
     attn, mlp = layer.self_attn, layer.mlp
     ln1, ln2 = layer.input_layernorm, layer.post_attention_layernorm
     projs = [attn.q_proj, attn.k_proj, attn.v_proj]
-    kc, vc = cache.key_cache[attn.layer_idx], cache.value_cache[attn.layer_idx]
+    attend = _decode_attend(attn, cache, pos, one_launch=True)
 
     def forward(hidden_states, *args, **kwargs):
         pe = kwargs.get("position_embeddings")
@@ -392,16 +570,7 @@ def _decode_layer_forward(layer, cache, pos: Tensor):
         ops = torch.ops.metal_liger
         q, k, v = ops.gemv_rmsnorm_multi(hidden_states, ln1.weight, float(ln1.eps),
                                          [p.weight for p in projs], [p.bias for p in projs])
-        cos, sin = pe
-        if kc.shape[2] <= 256:  # q/k prep and attention in one launch
-            out = ops.decode_qk_attention(q, k, v, attn.q_norm.weight, attn.k_norm.weight,
-                                          float(attn.q_norm.eps), float(attn.k_norm.eps), cos,
-                                          sin, kc, vc, pos, float(attn.scaling))
-        else:
-            q4 = ops.decode_qk_norm_rope(q, k, v, attn.q_norm.weight, attn.k_norm.weight,
-                                         float(attn.q_norm.eps), float(attn.k_norm.eps), cos,
-                                         sin, kc, vc, pos)
-            out = ops.decode_attention(q4, kc, vc, pos, 1, float(attn.scaling))
+        out = attend(q, k, v, *pe)
         h = ops.gemv_residual(out.reshape(B, S, -1), attn.o_proj.weight, attn.o_proj.bias,
                               hidden_states)
         act = ops.gemv_rmsnorm_swiglu(h, ln2.weight, float(ln2.eps), mlp.gate_proj.weight,
@@ -539,8 +708,20 @@ class MetalLigerGenerator:
             out = out + bias.float()
         return out.to(w.dtype)
 
+    def _sample(self, h: Tensor, uniform: Tensor, sampling: dict) -> Tensor:
+        """[B] ids drawn from the logits of [B, H] hidden states (0 where no
+        logit is a number: an id the decoder can be given)."""
+        from metal_liger_b200.ops.fused_sampling import fused_sample
+
+        w = self.head.weight
+        if h.shape[0] <= 2 and w.shape[1] % 8 == 0:  # one HBM pass over the head
+            logits = torch.ops.metal_liger.gemv(h.contiguous(), w, getattr(self.head, "bias", None))
+        else:
+            logits = self._logits(h)
+        return fused_sample(logits, uniform, **sampling)[0].clamp_(min=0)
+
     # ------------------------------------------------------------------
-    # Greedy decode on a CUDA graph.  One decode step is captured once and
+    # Greedy (or fused-sampling) decode on a CUDA graph.  One decode step is captured once and
     # replayed per token; it advances itself: the device scalar `pos` (the
     # position of the token fed in) drives the KV write (index_copy_), the
     # RoPE positions (a view of it) and the [B, 1, 1, max_len] boolean
@@ -563,7 +744,11 @@ class MetalLigerGenerator:
                                   else pos.view(1, 1).expand(B, 1))}
         h = self.decoder(input_ids=tok, attention_mask=mask, past_key_values=cache,
                          use_cache=True, return_dict=True, **extra).last_hidden_state[:, -1, :]
-        tok.copy_(self._greedy(h).view(B, 1))
+        if st["sampling"] is None:
+            tok.copy_(self._greedy(h).view(B, 1))
+        else:
+            uniform = st["uniform"].index_select(0, pos + 1).view(B)
+            tok.copy_(self._sample(h, uniform, st["sampling"]).view(B, 1))
         out.index_copy_(1, pos + 1, tok)
         pos.add_(1)
 
@@ -580,7 +765,8 @@ class MetalLigerGenerator:
     def _fingerprint(self):
         return tuple(p.data_ptr() for p in self.model.parameters())
 
-    def _state(self, B: int, L: int, dtype, dev) -> "_DecodeState":
+    def _state(self, B: int, L: int, dtype, dev, kv_cache_dtype: Optional[str] = None,
+               sampled: bool = False) -> "_DecodeState":
         """The static buffers (KV cache, ids, position, mask, input token)
         and, once captured, the decode graph for this (batch, length); kept
         across calls while the model's parameters stay where they are."""
@@ -588,10 +774,10 @@ class MetalLigerGenerator:
         if fp != getattr(self, "_states_fp", None):
             self._states = OrderedDict()
             self._states_fp = fp
-        key = (B, L, dtype, str(dev))
+        key = (B, L, dtype, str(dev), kv_cache_dtype, sampled)
         st = self._states.get(key)
         if st is None:
-            st = _DecodeState(self.model, B, L, dtype, dev)
+            st = _DecodeState(self.model, B, L, dtype, dev, kv_cache_dtype, sampled)
             self._states[key] = st
             while len(self._states) > self._MAX_STATES:
                 self._states.popitem(last=False)
@@ -607,9 +793,11 @@ class MetalLigerGenerator:
         HBM-streaming GEMV while the step is built (batch <= 2)."""
         B = st.ids.shape[0]
         if capture and st.graph is None:
-            with _DecodeKernels(self.decoder, st.pos, gemv=B <= 2, cache=st.cache):
+            with _DecodeKernels(self.decoder, st.pos, gemv=B <= 2, cache=st.cache), \
+                    _QuantizedAttention(self.decoder, st.cache):
                 return self._decode_static_inner(st, n, steps, eos_token_id, capture)
-        return self._decode_static_inner(st, n, steps, eos_token_id, capture)
+        with _QuantizedAttention(self.decoder, st.cache):
+            return self._decode_static_inner(st, n, steps, eos_token_id, capture)
 
     def _decode_static_inner(self, st: "_DecodeState", n, steps, eos_token_id,
                              capture: bool) -> int:
@@ -619,7 +807,8 @@ class MetalLigerGenerator:
         st.mask.zero_()
         st.mask[..., :n - 1] = True
         st.tok.copy_(ids[:, n - 1:n])
-        step = {"cache": cache, "tok": st.tok, "pos": st.pos, "mask": st.mask, "out": ids}
+        step = {"cache": cache, "tok": st.tok, "pos": st.pos, "mask": st.mask, "out": ids,
+                "sampling": st.sampling, "uniform": st.uniform}
         cache.graph_pos = st.pos
         done = 0
         try:
@@ -666,7 +855,10 @@ class MetalLigerGenerator:
     @torch.inference_mode()
     def generate(self, input_ids: Tensor, max_new_tokens: int = 128, temperature: float = 1.0,
                  top_p: float = 1.0, eos_token_id: Optional[int] = None,
-                 cuda_graph: Optional[bool] = None, **kwargs) -> Tensor:
+                 cuda_graph: Optional[bool] = None, *, kv_cache_dtype: Optional[str] = None,
+                 fused_sampling: bool = False, top_k: Optional[int] = None,
+                 min_p: Optional[float] = None,
+                 generator: Optional[torch.Generator] = None, **kwargs) -> Tensor:
         """Prefill the prompt, then decode one token per step (reference
         generation.py:74-129); returns [batch, prompt + generated] ids.
 
@@ -674,28 +866,51 @@ class MetalLigerGenerator:
         of text prompts on a CUDA device) decodes on a replayed CUDA graph of
         the step; the tokens are the same as the eager loop's up to
         near-ties at the logits' rounding (the attention then runs over the
-        full static buffers under a mask)."""
+        full static buffers under a mask).
+
+        The keyword-only arguments are not in the reference either.
+        ``kv_cache_dtype`` "int8" or "fp8" holds the KV cache in 8 bits.
+        ``fused_sampling`` (implied by ``top_k`` or ``min_p``) draws every token,
+        the first included, with ``ops.fused_sampling`` from ``temperature``,
+        ``top_k``, ``top_p`` and ``min_p``, all honoured (temperature 0 is
+        greedy), on the captured step as well; ``generator`` (a CUDA
+        ``torch.Generator``) gives its uniform numbers."""
         batch_size, prompt_len = input_ids.shape
         max_len = prompt_len + max_new_tokens
-        greedy = temperature == 0 or (temperature == 1.0 and top_p == 1.0)
+        fused = (fused_sampling or top_k is not None or min_p is not None) and temperature != 0
+        greedy = not fused and (temperature == 0 or (temperature == 1.0 and top_p == 1.0))
         if cuda_graph is None:
             cuda_graph = (input_ids.device.type == "cuda"
                           and max_new_tokens > self._GRAPH_WARMUP + 2)
-        static = greedy and not kwargs and cuda_graph and max_new_tokens > 1
+        sampling = uniform = None
+        if fused:
+            sampling = {"temperature": float(temperature), "top_k": int(top_k or 0),
+                        "top_p": float(top_p), "min_p": float(min_p or 0.0)}
+            _check_sampling(**sampling)
+            uniform = torch.rand((max_new_tokens, batch_size), generator=generator,
+                                 device=input_ids.device)
+        static = (greedy or fused) and not kwargs and cuda_graph and max_new_tokens > 1
         if static:
-            st = self._state(batch_size, max_len, input_ids.dtype, input_ids.device)
+            st = self._state(batch_size, max_len, input_ids.dtype, input_ids.device,
+                             kv_cache_dtype, fused)
             cache, ids = st.cache, st.ids
             cache.seen_tokens = 0
+            if fused:
+                for name, value in sampling.items():
+                    st.sampling[name].fill_(value)
+                st.uniform[prompt_len:] = uniform
         else:
-            cache = MetalLigerStaticCache(self.model, batch_size, max_len)
+            cache = _new_cache(self.model, batch_size, max_len, kv_cache_dtype)
             ids = torch.empty((batch_size, max_len), dtype=input_ids.dtype,
                               device=input_ids.device)
         ids[:, :prompt_len] = input_ids
 
-        # Prefill; the first token is the argmax in every mode (reference :99-101).
+        # Prefill; the first token is the argmax in every mode of the reference
+        # (:99-101).
         h = self._hidden_last(input_ids, cache, kwargs)
         cache.seen_tokens += prompt_len
-        next_token = self._greedy(h).to(ids.dtype).view(batch_size, 1)
+        first = self._sample(h, uniform[0], sampling) if fused else self._greedy(h)
+        next_token = first.to(ids.dtype).view(batch_size, 1)
         ids[:, prompt_len:prompt_len + 1] = next_token
         n = prompt_len + 1
 
@@ -704,12 +919,16 @@ class MetalLigerGenerator:
                                          capture=ids.device.type == "cuda")
             return ids[:, :filled].clone()
 
-        for _ in range(max_new_tokens - 1):
+        for step in range(1, max_new_tokens):
             if eos_token_id is not None and bool((next_token == eos_token_id).all()):
                 break
-            h = self._hidden_last(next_token, cache, kwargs)
+            with _QuantizedAttention(self.decoder, cache):
+                h = self._hidden_last(next_token, cache, kwargs)
             cache.seen_tokens += 1
-            if greedy:
+            if fused:
+                next_token = self._sample(h, uniform[step], sampling).to(ids.dtype).view(
+                    batch_size, 1)
+            elif greedy:
                 next_token = self._greedy(h).to(ids.dtype).view(batch_size, 1)
             else:
                 probs = torch.softmax(self._logits(h) / temperature, dim=-1)
@@ -719,18 +938,39 @@ class MetalLigerGenerator:
         return ids[:, :n]
 
 
+def _check_sampling(temperature: float, top_k: int, top_p: float, min_p: float) -> None:
+    if not (0.0 < temperature < float("inf") and top_k >= 0 and 0.0 <= top_p <= 1.0
+            and 0.0 <= min_p <= 1.0):
+        raise ValueError(f"generate: temperature={temperature}, top_k={top_k}, top_p={top_p}, "
+                         f"min_p={min_p}")
+
+
+def _new_cache(model: nn.Module, batch_size: int, max_len: int, kv_cache_dtype: Optional[str]):
+    if kv_cache_dtype is None:
+        return MetalLigerStaticCache(model, batch_size, max_len)
+    return MetalLigerQuantizedCache(model, batch_size, max_len, kv_cache_dtype)
+
+
 class _DecodeState:
     """Buffers of the self-advancing decode step for one (batch, length):
     the static KV cache, the [B, L] ids, the device position, the [B, 1, 1,
-    L] attention mask, the input token, and the captured graph (None until
-    the first call long enough to capture it)."""
+    L] attention mask, the input token, the sampler's per-row settings and the
+    uniform number of every position, and the captured graph (None until the
+    first call long enough to capture it)."""
 
-    def __init__(self, model: nn.Module, B: int, L: int, dtype, dev):
-        self.cache = MetalLigerStaticCache(model, B, L)
+    def __init__(self, model: nn.Module, B: int, L: int, dtype, dev,
+                 kv_cache_dtype: Optional[str] = None, sampled: bool = False):
+        self.cache = _new_cache(model, B, L, kv_cache_dtype)
         self.ids = torch.empty((B, L), dtype=dtype, device=dev)
         self.pos = torch.zeros(1, dtype=torch.int64, device=dev)
         self.mask = torch.zeros((B, 1, 1, L), dtype=torch.bool, device=dev)
         self.tok = torch.empty((B, 1), dtype=dtype, device=dev)
+        self.sampling = self.uniform = None
+        if sampled:
+            self.sampling = {n: torch.zeros(B, dtype=torch.float32, device=dev)
+                             for n in ("temperature", "top_p", "min_p")}
+            self.sampling["top_k"] = torch.zeros(B, dtype=torch.int64, device=dev)
+            self.uniform = torch.zeros((L, B), dtype=torch.float32, device=dev)
         self.graph = None
 
 

@@ -784,42 +784,46 @@ kv8_attention_kernel(const __grid_constant__ AttnArgs a) {
   cp_wait<0>();
   __syncthreads();
 
-  // Join the pieces: those of one segment follow one another.  A lane per
-  // entry finds the runs; then a warp per row makes the entries' factors with
-  // reductions inside the runs.
-  static_assert(2 * NW <= 32, "an entry per lane");
-  Piece mine = {0, 0, 0, 0, 0};
-  if (lane < 2 * NW) mine = pieces[lane];
-  const unsigned valid = __ballot_sync(0xffffffffu, mine.hi > 0);
+  // Join the pieces: those of one segment follow one another.  A group of a
+  // lane per entry finds the runs; then a group per row makes the entries'
+  // factors with reductions inside the runs.
+  constexpr int E = 2 * NW, kGroups = 32 / E;
+  static_assert(E <= 32, "a lane per entry");
+  const int e = lane % E, base = lane - e;
+  constexpr unsigned kEntries = E == 32 ? 0xffffffffu : (1u << E) - 1;
+  const Piece mine = pieces[e];
+  const unsigned valid = __ballot_sync(0xffffffffu, mine.hi > 0) & kEntries;
   if (valid == 0) return;
-  const unsigned below = (1u << lane) - 1, upto = below | (1u << lane);
-  const int prev = (valid & below) ? 31 - __clz(valid & below) : lane;
+  const unsigned below = (1u << e) - 1, upto = below | (1u << e);
+  const int prev = base + ((valid & below) ? 31 - __clz(valid & below) : e);
   const int prev_b = __shfl_sync(0xffffffffu, mine.b, prev);
   const int prev_seg = __shfl_sync(0xffffffffu, mine.seg, prev);
-  const bool starts = mine.hi > 0 && ((valid & below) == 0 || prev_b != mine.b || prev_seg != mine.seg);
-  const unsigned head = __ballot_sync(0xffffffffu, starts);
-  const int my_head = (head & upto) ? 31 - __clz(head & upto) : lane;
-  const int end = (head & ~upto) ? __ffs(head & ~upto) - 1 : 32;  // of this lane's run
+  const bool on = mine.hi > 0;
+  const bool starts = on && ((valid & below) == 0 || prev_b != mine.b || prev_seg != mine.seg);
+  const unsigned head = __ballot_sync(0xffffffffu, starts) & kEntries;
+  const int my_head = base + ((head & upto) ? 31 - __clz(head & upto) : e);
+  const int end = (head & ~upto) ? __ffs(head & ~upto) - 1 : E;  // of this entry's run
   const unsigned in_run = valid & (end == 32 ? 0xffffffffu : (1u << end) - 1);
   const int head_lo = __shfl_sync(0xffffffffu, mine.lo, my_head);
-  const int last_hi = __shfl_sync(0xffffffffu, mine.hi, in_run ? 31 - __clz(in_run) : 0);
+  const int last_hi = __shfl_sync(0xffffffffu, mine.hi, base + (in_run ? 31 - __clz(in_run) : 0));
   const bool whole = head_lo == 0 && last_hi == mine.tiles;
   const int rank = __popc(valid & below);
-  if (warp == 0 && mine.hi > 0) {
-    entry[rank] = lane;
+  if (threadIdx.x < E && on) {
+    entry[rank] = e;
     if (starts)
       runs[__popc(head & below)] = {rank, __popc(in_run), mine.b, mine.seg, whole, mine.lo > 0};
   }
-  for (int r = warp; r < C::kRows; r += NW) {
-    const bool on = mine.hi > 0;
-    const float m = on ? stats[lane][r] : -INFINITY;
-    const float l = on ? stats[lane][C::kRows + r] : 0.f;
-    const float mo = on ? stats[lane][2 * C::kRows + r] : -INFINITY;
+#pragma unroll 1
+  for (int r0 = warp * kGroups; r0 < C::kRows; r0 += NW * kGroups) {
+    const int r = r0 + lane / E;
+    const float m = on ? stats[e][r] : -INFINITY;
+    const float l = on ? stats[e][C::kRows + r] : 0.f;
+    const float mo = on ? stats[e][2 * C::kRows + r] : -INFINITY;
     float M = m, MO = mo;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < E; o <<= 1) {
       const float x = __shfl_down_sync(0xffffffffu, M, o), y = __shfl_down_sync(0xffffffffu, MO, o);
-      if (lane + o < end) {
+      if (e + o < end) {
         M = fmaxf(M, x);
         MO = fmaxf(MO, y);
       }
@@ -828,9 +832,9 @@ kv8_attention_kernel(const __grid_constant__ AttnArgs a) {
     MO = __shfl_sync(0xffffffffu, MO, my_head);
     float L = on ? l * rel2(m, M) : 0.f;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < E; o <<= 1) {
       const float x = __shfl_down_sync(0xffffffffu, L, o);
-      if (lane + o < end) L += x;
+      if (e + o < end) L += x;
     }
     L = __shfl_sync(0xffffffffu, L, my_head);
     if (on) {

@@ -26,10 +26,10 @@
 // is found by selection, not by sorting: a histogram over the distance to the
 // largest logit, of counts (top-k) or weights (top-p), gives the bin that the
 // prefix ends in.  The tokens from there up are few as a rule; they go, in
-// index order, to a list in the cluster's first CTA, which finishes alone.
-// Otherwise the steps go on over the slices.  Histograms over the bin's keys
-// narrow it to one key, the tokens equal to it are cut by index, and the draw
-// adds up kept weights by CTA, warp and lane in index order.
+// index order, to a list in the cluster's first CTA, which sorts it and draws.
+// Otherwise the steps go on over the slices: histograms over the bin's keys
+// narrow it to one key, and the draw adds up kept weights, and tokens equal to
+// that key as long as they are kept, by CTA, warp and lane in index order.
 //
 // Tokens that need fp64 are rare in most rows and everywhere in flat ones: a
 // warp queues them and weighs 32 at a time.
@@ -52,7 +52,7 @@ constexpr double kOne = 8796093022208.0;  // 2^43
 // A slice that leaves room for two CTAs on an SM is held; a larger one is read
 // again from L2 (256 fp32 rows: 107 us, against 145 held by one CTA per SM).
 constexpr size_t kMaxResident = 80 * 1024;
-constexpr int kList = 1024;          // tokens of the list
+constexpr int kList = kThreads;      // tokens of the list
 constexpr int kWarpList = kList / kWarps;  // of them from one warp
 constexpr int kTable = 64;
 
@@ -174,21 +174,24 @@ struct Row {
   }
 };
 
-// Which tokens are left: logit > x, or equal and index < end.  (NaN never is.)
+// Which tokens are left: the ones with a logit above x, and the first `ties` of
+// those equal to it.
 struct Cut {
-  float x = -INFINITY;
-  int end = -0x7fffffff;  // below the negative indices of what lies before the row, too
-  __device__ __forceinline__ bool has(float v, int i) const { return v > x || (v == x && i < end); }
+  static constexpr float kNone = -3.4028235e38f;  // (-inf and NaN never are)
+  float x = kNone;
+  uint64_t ties = ~(uint64_t)0;
+  __device__ __forceinline__ bool has(float v) const { return v >= x; }  // but for the ties
 };
 
 struct Shared {
   double table[kTable];            // 2^(i / kTable)
-  uint32_t hist[2][3][kBins];      // 15-bit parts of the sums, two in turn
-  uint64_t sums[kBins];            // over the cluster
-  uint64_t slot[10][kMaxCluster];  // one exchange each
+  uint32_t hist[3][kBins];         // 15-bit parts of the sums
+  uint64_t sums[2][kBins];         // this CTA's, for the others to read; two in turn
+  uint64_t slot[5][kMaxCluster];   // one exchange each
   uint64_t part[kWarps], walk[kWarps];
-  uint64_t above;
-  int bin, found;
+  int ties[kWarps];
+  uint64_t above, in_bin;
+  int bin;
   uint32_t key[2];
   float queue[kWarps][64];
   float list_x[kList];
@@ -222,18 +225,8 @@ struct Slice {
   }
   __device__ __forceinline__ int index(int v) const { return base + v * N; }
 };
-// The list, a token at a time.
-struct List {
-  static constexpr int N = 1;
-  const float* x_;
-  const int* i_;
-  int count;
-  __device__ __forceinline__ void get(int v, float* x) const { x[0] = x_[v]; }
-  __device__ __forceinline__ int index(int v) const { return i_[v]; }
-};
-
-// Calls f(active, x[N], index) for the tokens of this warp's share of the
-// source, all lanes together; lanes interleave, so a lane's tokens ascend.
+// Calls f(x[N], index) for the tokens of this warp's share of the slice, all
+// lanes together; lanes interleave, so a lane's tokens ascend.
 template <typename S, typename F>
 __device__ __forceinline__ void each(const S& src, F&& f) {
   const int per = (src.count + kWarps - 1) / kWarps, warp = threadIdx.x >> 5;
@@ -255,19 +248,21 @@ __device__ __forceinline__ void each(const S& src, F&& f) {
 
 // each() for weights: sink(x, W, valid) gets the large ones, a warp at a time;
 // the sum of this lane's small ones is returned.  OPEN: the cut has everything.
-template <bool OPEN, typename S, typename R, typename F>
+// TIES: this lane's tokens equal to the cut's x are counted.
+template <bool OPEN, bool TIES, typename S, typename R, typename F>
 __device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, const Cut& cut,
-                                                float* queue, F&& sink) {
+                                                float* queue, int* ties, F&& sink) {
   const int lane = threadIdx.x & 31;
   const unsigned before = (1u << lane) - 1;
   uint64_t tail = 0;
   int waiting = 0, at = 0;
-  each(src, [&](const float* x, int i) {
+  each(src, [&](const float* x, int) {
     uint32_t small = 0, large = 0;
 #pragma unroll
     for (int e = 0; e < S::N; ++e) {
       // (-inf and NaN take the floor's place, which weighs nothing)
-      const bool in = OPEN || cut.has(x[e], i + e);
+      const bool in = OPEN || cut.has(x[e]);
+      if (TIES) *ties += x[e] == cut.x;
       const float y = fmaxf(x[e], row.floor), z = row.log2_weight(y);
       const uint32_t w = row.small_weight(y, z);
       if (!R::small(z)) large |= in ? 1u << e : 0;
@@ -351,80 +346,15 @@ __device__ __forceinline__ void add_warp(uint32_t (*hist)[kBins], int bin, uint6
   }
 }
 
-// What the draw and the cut by index share: `mine` is the sum of this warp's
-// share of the source, value(x, i) that of one token.  Finds the first token, in
-// index order, at which the running sum over the cluster passes `want` (OVER) or
-// reaches it.  Returns its index in the CTA that has it, -1 in the others and
-// where the sum does not get there.  FRACTION: want is a fraction of the total.
-template <bool OVER, bool FRACTION, typename S, typename F>
-__device__ int locate(const S& src, const Cluster& cl, Shared& sh, int step, double want,
-                      uint64_t mine, F&& value, uint64_t* total_out) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();
-  if (lane == 0) sh.part[warp] = mine;
-  if (threadIdx.x == 0) sh.found = -1;
-  __syncthreads();
-  uint64_t here = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) here += sh.part[w];
-  cl.gather(sh, step, here);
-  uint64_t before = 0, total = 0;
-  for (int r = 0; r < cl.size; ++r) {
-    if (r < cl.rank) before += sh.slot[step][r];
-    total += sh.slot[step][r];
-  }
-  *total_out = total;
-  const double target = FRACTION ? want * (double)total : want;
-  auto reached = [&](uint64_t s) { return OVER ? (double)s > target : (double)s >= target; };
-  if (reached(before) || !reached(before + here)) return -1;
-  // this CTA: the warp whose share it is, then a thread per vector of that share
-  uint64_t run = before;
-  int w = 0;
-  while (w < kWarps - 1 && !reached(run + sh.part[w])) run += sh.part[w++];
-  const int per = (src.count + kWarps - 1) / kWarps, end = min(src.count, (w + 1) * per);
-  for (int v0 = w * per; v0 < end; v0 += kThreads) {
-    const int v = v0 + threadIdx.x;
-    float x[S::N];
-    uint64_t s = 0;
-    int i = 0;
-    if (v < end) {
-      src.get(v, x);
-      i = src.index(v);
-#pragma unroll
-      for (int e = 0; e < S::N; ++e) s += value(x[e], i + e);
-    }
-    uint64_t incl = warp_scan64(s), all = 0;
-    if (lane == 31) sh.walk[warp] = incl;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) {
-      if (j < warp) incl += sh.walk[j];
-      all += sh.walk[j];
-    }
-    uint64_t at = run + incl - s;
-    if (s > 0 && !reached(at) && reached(at + s)) {
-#pragma unroll
-      for (int e = 0; e < S::N; ++e) {
-        const uint64_t c = value(x[e], i + e);
-        if (c > 0 && !reached(at) && reached(at + c)) sh.found = i + e;
-        at += c;
-      }
-    }
-    run += all;
-    __syncthreads();
-    if (sh.found >= 0) break;
-  }
-  return sh.found;
-}
-
 // Where a selection stands: the prefix ends among the keys [lo, hi], after
 // values of `above` before them; `need` in all.
 struct Search {
   uint32_t lo, hi;
   uint64_t above, need;
-  int round;    // histograms so far (of the two in turn)
-  bool whole;   // nothing to cut
-  bool beyond;  // the last histogram's last bin
+  int round;        // histograms so far (of the two sums in turn)
+  bool whole;       // nothing to cut
+  bool beyond;      // the prefix ends in the last histogram's last bin
+  uint64_t in_bin;  // sum of the bin that it ends in
 };
 
 // What a histogram's bins are: distances to the top, near or far, or keys.
@@ -433,58 +363,57 @@ struct Search {
 enum Bins { kNear, kFar, kKeys };
 
 // One histogram of the tokens in `in` and [q.lo, q.hi]; q narrows to the bin
-// that the prefix ends in.  WEIGHT: q.need, where 0, becomes p of the sum.
+// that the prefix ends in.  WEIGHT: q.need, where 0, becomes p of the sum less
+// `excess`, the weight of the last tokens in the order that are not in `in`.
 template <bool WEIGHT, Bins BINS, typename S, typename R>
 __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row, const Cut& in,
-                       Search& q, double p) {
+                       Search& q, double p, uint64_t excess) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kFrom = BINS == kFar ? kBins / 2 : 0;
   const float per = (WEIGHT ? row.rate_f * 32.f : 16.f) * (BINS == kFar ? 0.5f : 1.f);
   auto distance = [&](float x) {
     // (NaN, at the top where it or the rate is infinite, converts to 0)
-    const int d = __float2int_rz((row.top - x) * per) - (BINS == kFar ? kBins / 2 : 0);
-    return max(0, min(d, kBins - 1));
+    return max(0, min(__float2int_rz((row.top - x) * per) - kFrom, kBins - 1));
   };
   const int bits = 32 - __clz(q.hi - q.lo);
   const int shift = bits > 9 ? bits - 9 : 0;
-  uint32_t (*hist)[kBins] = sh.hist[q.round & 1];
 #pragma unroll
-  for (int i = 0; i < 3; ++i) hist[i][tid] = 0;
+  for (int i = 0; i < 3; ++i) sh.hist[i][tid] = 0;
   __syncthreads();
+  if (tid == 0) sh.bin = kBins - 1;
   if (WEIGHT && BINS == kNear) {
-    uint64_t tail = each_weight<false>(src, row, in, sh.queue[warp], [&](float x, uint64_t w, bool valid) {
-      add_warp(hist, distance(x), w, valid);
-    });
+    uint64_t tail = each_weight<false, false>(
+        src, row, in, sh.queue[warp], nullptr,
+        [&](float x, uint64_t w, bool valid) { add_warp(sh.hist, distance(x), w, valid); });
     tail = warp_sum64(tail);  // small ones are past 18 log2s: all in the last bin
-    if (lane == 0) add_parts(hist, kBins - 1, tail);
+    if (lane == 0) add_parts(sh.hist, kBins - 1, tail);
   } else {
     // in the keys' range by value: -0 has a key of its own, which no token has
     constexpr uint32_t kMinusZero = 0x7fffffffu >> R::kKey;
-    const float x_lo = value_of<R::kKey>(q.lo == kMinusZero ? q.lo + 1 : q.lo);
+    const float x_lo = fmaxf(value_of<R::kKey>(q.lo == kMinusZero ? q.lo + 1 : q.lo), in.x);
     const float x_hi = value_of<R::kKey>(q.hi == kMinusZero ? q.hi - 1 : q.hi);
-    each(src, [&](const float* x, int i) {
+    each(src, [&](const float* x, int) {
 #pragma unroll
       for (int e = 0; e < S::N; ++e) {
-        if (!(x[e] >= x_lo && x[e] <= x_hi) || !in.has(x[e], i + e)) continue;
+        if (!(x[e] >= x_lo && x[e] <= x_hi)) continue;
         const int bin =
             BINS == kKeys ? (int)((q.hi - key_of<R::kKey>(x[e])) >> shift) : distance(x[e]);
-        if (WEIGHT) add_parts(hist, bin, row.weight(x[e]));
-        else atomicAdd(&hist[0][bin], 1u);
+        if (WEIGHT) add_parts(sh.hist, bin, row.weight(x[e]));
+        else atomicAdd(&sh.hist[0][bin], 1u);
       }
     });
   }
-  cl.sync();
-  {
-    // a thread per bin of this CTA's share and CTA that counted it
-    const int r = tid % cl.size, bin = cl.rank * (kBins / cl.size) + tid / cl.size;
-    const uint32_t (*h)[kBins] = cl.of(&sh, r)->hist[q.round & 1];
-    uint64_t v = h[0][bin] + ((uint64_t)h[1][bin] << 15) + ((uint64_t)h[2][bin] << 30);
-    for (int o = cl.size / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    cl.of(&sh, r)->sums[bin] = v;
+  __syncthreads();
+  uint64_t s = sh.hist[0][tid] + ((uint64_t)sh.hist[1][tid] << 15) + ((uint64_t)sh.hist[2][tid] << 30);
+  if (cl.size > 1) {
+    uint64_t* mine = &sh.sums[q.round & 1][tid];
+    *mine = s;
+    cl.sync();
+    s = 0;
+#pragma unroll 8
+    for (int r = 0; r < cl.size; ++r) s += *cl.of(mine, r);
   }
   ++q.round;
-  if (tid == 0) sh.bin = kBins - 1;
-  cl.sync();
-  const uint64_t s = sh.sums[tid];
   uint64_t incl = warp_scan64(s);
   if (lane == 31) sh.part[warp] = incl;
   __syncthreads();
@@ -495,6 +424,7 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
     total += sh.part[w];
   }
   if (BINS == kNear) {
+    total -= excess;
     if (WEIGHT && q.need == 0) {
       const double f = ceil(p * (double)total);
       q.need = f < 1.0 ? 1 : (uint64_t)f;
@@ -507,10 +437,12 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
   if (q.above + incl >= q.need && q.above + incl - s < q.need) {
     sh.bin = tid;
     sh.above = q.above + incl - s;
+    sh.in_bin = s;
   }
   __syncthreads();
   const int bin = sh.bin;
   q.above = sh.above;
+  q.in_bin = sh.in_bin;
   q.beyond = bin == kBins - 1;
   if (BINS == kKeys) {
     const uint64_t down = (uint64_t)bin << shift;
@@ -521,18 +453,30 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
     return;
   }
   // The keys of a bin of distances are neighbours: find the first and last
-  // (distances fall as keys grow) by 32-way search, a warp for each: the
-  // smallest key with a distance <= bin, and < bin.
+  // (distances fall as keys grow), a warp for each: the smallest key with a
+  // distance <= bin, and < bin.  By 32-way search, from around the bin's edge
+  // where that holds the key.
   if (warp < 2) {
+    auto holds = [&](uint64_t k) {
+      const int d = distance(value_of<R::kKey>((uint32_t)k));
+      return warp == 0 ? d <= bin : d < bin;
+    };
     uint32_t a = q.lo, b = q.hi + 1;  // the answer lies in [a, b]
+    const float edge = row.top - (float)(bin + kFrom + 1 - warp) / per;
+    const float off = (fabsf(row.top) + fabsf(edge)) * 1e-6f;
+    if (off < 1e30f) {
+      const uint32_t ka = key_of<R::kKey>(edge - off), kb = key_of<R::kKey>(edge + off) + 1;
+      const bool inside = ka > a && kb < b && ka < kb;
+      if (__ballot_sync(0xffffffffu, inside && (lane == 0 ? !holds(ka - 1) : holds(kb))) ==
+          0xffffffffu) {
+        a = ka;
+        b = kb;
+      }
+    }
     while (a < b) {
       const uint32_t step = (b - a + 31) / 32;
       const uint64_t k = (uint64_t)a + (uint64_t)step * lane;
-      bool ok = k >= b;
-      if (!ok) {
-        const int d = distance(value_of<R::kKey>((uint32_t)k));
-        ok = warp == 0 ? d <= bin : d < bin;
-      }
+      const bool ok = k >= b || holds(k);
       const unsigned m = __ballot_sync(0xffffffffu, ok);
       const int f = m ? __ffs(m) - 1 : 32;
       const uint64_t t = (uint64_t)a + (uint64_t)step * f;
@@ -550,36 +494,22 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
 // The histograms by distance; false where they go past the near ones.
 template <bool WEIGHT, typename S, typename R>
 __device__ bool begin(const S& src, const Cluster& cl, Shared& sh, const R& row, const Cut& in,
-                      Search& q, double p) {
-  narrow<WEIGHT, kNear>(src, cl, sh, row, in, q, p);
+                      Search& q, double p, uint64_t excess) {
+  narrow<WEIGHT, kNear>(src, cl, sh, row, in, q, p, excess);
   if (q.whole || !q.beyond) return true;
-  narrow<WEIGHT, kFar>(src, cl, sh, row, in, q, p);
+  narrow<WEIGHT, kFar>(src, cl, sh, row, in, q, p, excess);
   return false;
 }
 
-// Narrows to one key and cuts the tokens equal to it by index.
+// Narrows to one key; as many of the tokens equal to it are left as still needed.
 template <bool WEIGHT, typename S, typename R>
 __device__ Cut finish(const S& src, const Cluster& cl, Shared& sh, const R& row, const Cut& in,
-                      Search& q, int step) {
-  while (q.lo < q.hi) narrow<WEIGHT, kKeys>(src, cl, sh, row, in, q, 0.0);
-  // as many as are still needed, lowest index first
-  const float x = value_of<R::kKey>(q.lo);
-  const uint64_t each_w = WEIGHT ? row.weight(x) : 1;
-  const uint64_t want = (q.need - q.above + each_w - 1) / each_w;
-  auto value = [&](float v, int i) -> uint64_t { return v == x && in.has(v, i); };
-  uint64_t mine = 0, ties;
-  each(src, [&](const float* v, int i) {
-#pragma unroll
-    for (int e = 0; e < S::N; ++e) mine += value(v[e], i + e);
-  });
-  mine = warp_sum64(mine);
-  const int at = locate<false, false>(src, cl, sh, step, (double)want, mine, value, &ties);
-  // one CTA found it, all learn it
-  cl.gather(sh, step + 1, (uint64_t)(int64_t)at);
+                      Search& q) {
+  while (q.lo < q.hi) narrow<WEIGHT, kKeys>(src, cl, sh, row, in, q, 0.0, 0);
   Cut c;
-  c.x = x;
-  c.end = 0;
-  for (int r = 0; r < cl.size; ++r) c.end = max(c.end, (int)(int64_t)sh.slot[step + 1][r] + 1);
+  c.x = value_of<R::kKey>(q.lo);
+  const uint64_t each_w = WEIGHT ? row.weight(c.x) : 1;
+  c.ties = (q.need - q.above + each_w - 1) / each_w;
   return c;
 }
 
@@ -639,11 +569,11 @@ __device__ int collect(const Slice<T>& sl, const Cluster& cl, Shared& sh, float 
     kx[j] = hx[j * 32 + lane];
     ki[j] = hi[j * 32 + lane];
   }
-  cl.gather(sh, 7, fits ? (uint64_t)here : (uint64_t)kList + 1);
+  cl.gather(sh, 4, fits ? (uint64_t)here : (uint64_t)kList + 1);
   int before = 0, total = 0;
   for (int r = 0; r < cl.size; ++r) {
-    if (r < cl.rank) before += (int)sh.slot[7][r];
-    total += (int)sh.slot[7][r];
+    if (r < cl.rank) before += (int)sh.slot[4][r];
+    total += (int)sh.slot[4][r];
   }
   if (total > kList) return -1;
   Shared* to = cl.of(&sh, 0);
@@ -665,20 +595,27 @@ struct Filter {
 };
 
 // Inclusive sums over the CTA, and the whole.
-__device__ __forceinline__ uint64_t block_scan(Shared& sh, uint64_t v, uint64_t* total) {
+__device__ __forceinline__ uint64_t block_scan(Shared& sh, uint64_t v, uint64_t* total,
+                                               uint64_t* part) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_scan64(v);
   __syncthreads();
-  if (lane == 31) sh.part[warp] = v;
+  if (lane == 31) part[warp] = v;
   __syncthreads();
   uint64_t all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) v += sh.part[w];
-    all += sh.part[w];
+    if (w < warp) v += part[w];
+    all += part[w];
   }
   *total = all;
   return v;
+}
+
+// u of the total, below it: the token is the first with a running weight above.
+__device__ __forceinline__ uint64_t target_of(const Filter& f, uint64_t total) {
+  const double t = (f.u > 0.f ? (double)f.u : 0.0) * (double)total;
+  return t < (double)total ? min((uint64_t)t, total - 1) : total - 1;
 }
 
 // The list's n <= kThreads tokens, a thread each: sorted, cut by rank and running
@@ -700,9 +637,9 @@ __device__ void draw_sorted(Shared& sh, const R& row, const Filter& f, int n, ui
         other = __shfl_xor_sync(0xffffffffu, mine, j);
       } else {
         __syncthreads();
-        sh.sums[tid] = mine;
+        sh.sums[0][tid] = mine;
         __syncthreads();
-        other = sh.sums[tid ^ j];
+        other = sh.sums[0][tid ^ j];
       }
       const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
       if ((mine < other) == larger) mine = other;
@@ -711,10 +648,10 @@ __device__ void draw_sorted(Shared& sh, const R& row, const Filter& f, int n, ui
   const bool on = mine != 0 && tid < n;
   const int at = on ? (int)~(uint32_t)mine : 0;
   __syncthreads();
-  sh.sums[tid] = 0;
+  sh.sums[0][tid] = 0;
   const float x = on ? value_of<0>((uint32_t)(mine >> 32)) : row.top;
   uint64_t w = on && (f.k <= 0 || tid < f.k) ? row.weight(x) : 0, total;
-  const uint64_t upto = block_scan(sh, w, &total);
+  const uint64_t upto = block_scan(sh, w, &total, sh.part);
   if (f.p < 1.0) {
     if (need == 0) {
       const double c = ceil(f.p * (double)total);
@@ -723,95 +660,107 @@ __device__ void draw_sorted(Shared& sh, const R& row, const Filter& f, int n, ui
     if (upto - w >= need) w = 0;
   }
   if (f.least > 0.f && tid > 0 && !(row.exact(x) >= (double)f.least)) w = 0;
-  if (on) sh.sums[at] = w;
+  if (on) sh.sums[0][at] = w;
   __syncthreads();
-  w = sh.sums[tid];
-  const uint64_t run = block_scan(sh, w, &total);
-  if (tid == 0) sh.found = -1;
-  __syncthreads();
-  const double target = (f.u > 0.f ? (double)f.u : 0.0) * (double)total;
-  // (the last one where u is at or past 1, or rounded to it)
-  const bool end = target >= (double)total;
-  if (w > 0 && (end ? run == total : (double)run > target && !((double)(run - w) > target)))
-    write(sh.list_i[tid], total);
+  w = sh.sums[0][tid];
+  const uint64_t run = block_scan(sh, w, &total, sh.part);
+  const uint64_t target = target_of(f, total);
+  if (run > target && run - w <= target) write(sh.list_i[tid], total);
 }
 
 // Cuts and draws from `src`, whose tokens are in `in`; `q` is the selection that
 // has begun on the first of the two cuts that are on.  first: top index.
+// Draws from the slices' tokens in `cut`.
 template <typename S, typename R, typename W>
-__device__ void cut_and_draw(const S& src, const Cluster& cl, Shared& sh, const R& row,
-                             const Filter& f, Cut cut, uint32_t top_key, Search q, bool begun,
-                             W&& write) {
+__device__ void draw(const S& src, const Cluster& cl, Shared& sh, const R& row, const Filter& f,
+                     const Cut& cut, W&& write) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Search fresh = {kLowest<R::kKey>, top_key, 0, 0, q.round, false, false};
-  if (f.k > 0 && f.k < f.V) {
-    if (!begun) {
-      q = fresh;
-      q.need = (uint64_t)f.k;
-      begin<false>(src, cl, sh, row, cut, q, 0.0);
-    }
-    begun = false;
-    if (!q.whole) cut = finish<false>(src, cl, sh, row, cut, q, 1);
-  }
-  if (f.p < 1.0) {
-    if (!begun) {
-      const int round = q.round;
-      q = fresh;
-      q.round = round;
-      begin<true>(src, cl, sh, row, cut, q, f.p);
-    }
-    if (!q.whole) cut = finish<true>(src, cl, sh, row, cut, q, 3);
-  }
-  // min-p: the smallest logit whose weight is large enough, by 32-way search
-  if (f.least > 0.f) {
-    if (warp == 0) {
-      uint32_t lo = kLowest<R::kKey>, hi = top_key;  // the answer lies in [lo, hi]: the largest qualifies
-      while (lo < hi) {
-        const uint32_t step = (hi - lo + 31) / 32;
-        const uint64_t k = (uint64_t)lo + (uint64_t)step * lane;
-        const bool ok = k >= hi || row.exact(value_of<R::kKey>((uint32_t)k)) >= (double)f.least;
-        const unsigned m = __ballot_sync(0xffffffffu, ok);
-        const int j = m ? __ffs(m) - 1 : 32;
-        const uint64_t t = (uint64_t)lo + (uint64_t)step * j;
-        const uint32_t nh = t < hi ? (uint32_t)t : hi;
-        lo = j == 0 ? nh : (uint32_t)((uint64_t)lo + (uint64_t)step * (j - 1) + 1);
-        hi = nh;
-      }
-      if (lane == 0) sh.key[0] = lo;
-    }
-    __syncthreads();
-    const float x = value_of<R::kKey>(sh.key[0]);
-    if (x > cut.x) {
-      cut.x = x;
-      cut.end = 0x7fffffff;
-    }
-  }
-  uint64_t large = 0, total;
+  uint64_t large = 0;
+  int ties = 0;
   auto add = [&](float, uint64_t w, bool valid) { large += valid ? w : 0; };
-  const uint64_t small = cut.x == -INFINITY ? each_weight<true>(src, row, cut, sh.queue[warp], add)
-                                            : each_weight<false>(src, row, cut, sh.queue[warp], add);
+  const bool some = cut.ties != ~(uint64_t)0;  // of the tokens equal to cut.x
+  const uint64_t small =
+      some ? each_weight<false, true>(src, row, cut, sh.queue[warp], &ties, add)
+      : cut.x == Cut::kNone ? each_weight<true, false>(src, row, cut, sh.queue[warp], &ties, add)
+                            : each_weight<false, false>(src, row, cut, sh.queue[warp], &ties, add);
   const uint64_t mine = warp_sum64(small + large);
-  auto value = [&](float x, int i) -> uint64_t { return cut.has(x, i) ? row.weight(x) : 0; };
-  const double u = f.u > 0.f ? (double)f.u : 0.0;
-  const int id = locate<true, true>(src, cl, sh, 5, u, mine, value, &total);
-  if (id >= 0 && threadIdx.x == 0) write(id, total);
-  // (a CTA may leave from here on: what follows is for all or for none)
-  if (u * (double)total >= (double)total) {
-    // u at or past 1 (or rounded to it): the last kept token
-    int last = -1;
-    each(src, [&](const float* x, int i) {
-#pragma unroll 1
-      for (int e = 0; e < S::N; ++e)
-        if (value(x[e], i + e) > 0) last = i + e;
-    });
-    last = __reduce_max_sync(0xffffffffu, last);
-    __syncthreads();
-    if (lane == 0) sh.part[warp] = (uint64_t)(int64_t)last;
-    __syncthreads();
-    for (int i = 0; i < kWarps; ++i) last = max(last, (int)(int64_t)sh.part[i]);
-    cl.gather(sh, 6, (uint64_t)(int64_t)last);
-    for (int i = 0; i < cl.size; ++i) last = max(last, (int)(int64_t)sh.slot[6][i]);
-    if (cl.rank == 0 && threadIdx.x == 0) write(last, total);
+  ties = (int)__reduce_add_sync(0xffffffffu, (unsigned)ties);
+  const uint64_t each_w = some ? row.weight(cut.x) : 0;
+  __syncthreads();
+  if (lane == 0) {
+    sh.part[warp] = mine;
+    sh.ties[warp] = ties;
+  }
+  __syncthreads();
+  uint64_t here = 0, here_ties = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    here += sh.part[w];
+    here_ties += sh.ties[w];
+  }
+  if ((int)threadIdx.x < cl.size) {
+    cl.of(&sh, threadIdx.x)->slot[2][cl.rank] = here;
+    cl.of(&sh, threadIdx.x)->slot[3][cl.rank] = here_ties;
+  }
+  cl.sync();  // (nothing is exchanged any more: a CTA may leave)
+  // the ties that are kept go to the first CTAs that have any
+  uint64_t before = 0, total = 0, left = cut.ties, my_left = 0;
+  for (int r = 0; r < cl.size; ++r) {
+    const uint64_t n = sh.slot[3][r], kept = min(n, left);
+    const uint64_t w = sh.slot[2][r] - (n - kept) * each_w;
+    if (r < cl.rank) before += w;
+    if (r == cl.rank) {
+      here = w;
+      my_left = left;
+    }
+    total += w;
+    left -= kept;
+  }
+  const uint64_t target = target_of(f, total);
+  if (target < before || target >= before + here) return;
+  // this CTA: the warp whose share it is, then a thread per vector of that share
+  uint64_t run = before;
+  int w = 0;
+  for (; w < kWarps - 1; ++w) {
+    const uint64_t n = sh.ties[w], kept = min(n, my_left);
+    const uint64_t c = sh.part[w] - (n - kept) * each_w;
+    if (run + c > target) break;
+    run += c;
+    my_left -= kept;
+  }
+  const int per = (src.count + kWarps - 1) / kWarps, end = min(src.count, (w + 1) * per);
+  for (int v0 = w * per; v0 < end && run <= target; v0 += kThreads) {
+    const int v = v0 + threadIdx.x;
+    float x[S::N];
+    if (v < end) {
+      src.get(v, x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < S::N; ++e) x[e] = -INFINITY;
+    }
+    uint64_t rank = 0, all_ties = 0;  // of this thread's first tie
+    if (some) {
+#pragma unroll
+      for (int e = 0; e < S::N; ++e) rank += x[e] == cut.x;
+      const uint64_t n = rank;
+      rank = block_scan(sh, rank, &all_ties, sh.walk) - n;
+    }
+    uint64_t c[S::N], s = 0, all;
+#pragma unroll
+    for (int e = 0; e < S::N; ++e) {
+      const bool tie = some && x[e] == cut.x;
+      c[e] = cut.has(x[e]) && !(tie && rank >= my_left) ? row.weight(x[e]) : 0;
+      rank += tie;
+      s += c[e];
+    }
+    uint64_t at = run + block_scan(sh, s, &all, sh.walk) - s;
+#pragma unroll
+    for (int e = 0; e < S::N; ++e) {
+      if (at <= target && target < at + c[e]) write(src.index(v) + e, total);
+      at += c[e];
+    }
+    run += all;
+    my_left -= min(my_left, all_ties);
   }
 }
 
@@ -892,11 +841,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     return;  // every exchange is done
   }
   Row<G> row;
-  Cut all;
-  if (!row.set(value_of<G>(top_key), t, sh.table)) {
-    all.x = row.top;
-    all.end = 0x7fffffff;
-  }
+  Cut cut;
+  if (!row.set(value_of<G>(top_key), t, sh.table)) cut.x = row.top;
 
   auto write = [&](int i, uint64_t total) {
     const float x = to_f32(sl.row[i]);
@@ -904,32 +850,58 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     a.id[r] = i;
     a.logprob[r] = (float)(z - log((double)total / kOne));
   };
-  // The first cut's first histogram; what lies from its bin up may fit the list.
-  Search q = {kLowest<G>, top_key, 0, 0, 0, false, false};
-  const bool by_count = f.k > 0 && f.k < a.V, by_weight = f.p < 1.0;
-  bool begun = false;
-  if (by_count || by_weight) {
-    begun = true;
-    bool near;  // far ones are many
-    if (by_count) {
-      q.need = (uint64_t)f.k;
-      near = begin<false>(sl, cl, sh, row, all, q, 0.0);
-    } else {
-      near = begin<true>(sl, cl, sh, row, all, q, f.p);
-    }
-    if (!q.whole && near) {
-      const int n = collect(sl, cl, sh, fmaxf(value_of<G>(q.lo), all.x));
-      if (n >= 0) {
-        if (cl.rank == 0) {
-          const List list = {sh.list_x, sh.list_i, n};
-          if (n <= kThreads) draw_sorted(sh, row, f, n, by_count ? 0 : q.need, write);
-          else cut_and_draw(list, Cluster{1, 0}, sh, row, f, all, top_key, q, begun, write);
-        }
-        return;  // nothing of the other CTAs is needed any more
-      }
+  // Each cut's first histogram; what lies from the first one's bin up may fit the
+  // list (far tokens are many).
+  auto listed = [&](const Search& q, uint64_t need) {
+    const int n = collect(sl, cl, sh, fmaxf(value_of<G>(q.lo), cut.x));
+    if (n >= 0 && cl.rank == 0) draw_sorted(sh, row, f, n, need, write);
+    return n >= 0;  // nothing of the other CTAs is needed any more
+  };
+  Search q = {kLowest<G>, top_key, 0, 0, 0, false, false, 0};
+  const bool by_count = f.k > 0 && f.k < a.V;
+  uint64_t excess = 0;
+  if (by_count) {
+    q.need = (uint64_t)f.k;
+    const bool near = begin<false>(sl, cl, sh, row, cut, q, 0.0, 0);
+    if (!q.whole) {
+      if (near && listed(q, 0)) return;
+      cut = finish<false>(sl, cl, sh, row, cut, q);
+      excess = (q.in_bin - cut.ties) * row.weight(cut.x);
     }
   }
-  cut_and_draw(sl, cl, sh, row, f, all, top_key, q, begun, write);
+  if (f.p < 1.0) {
+    q = {kLowest<G>, top_key, 0, 0, q.round, false, false, 0};
+    const bool near = begin<true>(sl, cl, sh, row, cut, q, f.p, excess);
+    if (!q.whole) {
+      if (!by_count && near && listed(q, q.need)) return;
+      cut = finish<true>(sl, cl, sh, row, cut, q);
+    }
+  }
+  // min-p: the smallest logit whose weight is large enough, by 32-way search
+  if (f.least > 0.f) {
+    if (warp == 0) {
+      uint32_t lo = kLowest<G>, hi = top_key;  // the answer lies in [lo, hi]: the largest qualifies
+      while (lo < hi) {
+        const uint32_t step = (hi - lo + 31) / 32;
+        const uint64_t k = (uint64_t)lo + (uint64_t)step * lane;
+        const bool ok = k >= hi || row.exact(value_of<G>((uint32_t)k)) >= (double)f.least;
+        const unsigned m = __ballot_sync(0xffffffffu, ok);
+        const int j = m ? __ffs(m) - 1 : 32;
+        const uint64_t top_k = (uint64_t)lo + (uint64_t)step * j;
+        const uint32_t nh = top_k < hi ? (uint32_t)top_k : hi;
+        lo = j == 0 ? nh : (uint32_t)((uint64_t)lo + (uint64_t)step * (j - 1) + 1);
+        hi = nh;
+      }
+      if (lane == 0) sh.key[0] = lo;
+    }
+    __syncthreads();
+    const float x = value_of<G>(sh.key[0]);
+    if (x > cut.x) {
+      cut.x = x;
+      cut.ties = ~(uint64_t)0;
+    }
+  }
+  draw(sl, cl, sh, row, f, cut, write);
 }
 
 // CTAs per row.  Few rows: eight, so that a row's passes are short (clusters of

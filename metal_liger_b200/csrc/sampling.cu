@@ -224,9 +224,12 @@ struct Slice {
     for (int e = 0; e < N; ++e) x[e] = to_f32(r.v[e]);
   }
   __device__ __forceinline__ int index(int v) const { return base + v * N; }
+  __device__ __forceinline__ float one(int v, int e) const {  // of a token of the row
+    return to_f32(held ? reinterpret_cast<const T*>(held)[v * N + e] : row[index(v) + e]);
+  }
 };
-// Calls f(x[N], index) for the tokens of this warp's share of the slice, all
-// lanes together; lanes interleave, so a lane's tokens ascend.
+// Calls f(x[N], v) for the vectors of this warp's share of the slice, all lanes
+// together; lanes interleave, so a lane's tokens ascend.
 template <typename S, typename F>
 __device__ __forceinline__ void each(const S& src, F&& f) {
   const int per = (src.count + kWarps - 1) / kWarps, warp = threadIdx.x >> 5;
@@ -234,15 +237,13 @@ __device__ __forceinline__ void each(const S& src, F&& f) {
   for (int v0 = begin; v0 < end; v0 += 32) {
     const int v = v0 + (threadIdx.x & 31);
     float x[S::N];
-    int i = 0;
     if (v < end) {
       src.get(v, x);
-      i = src.index(v);
     } else {
 #pragma unroll
       for (int e = 0; e < S::N; ++e) x[e] = -INFINITY;
     }
-    f(x, i);
+    f(x, v);
   }
 }
 
@@ -256,7 +257,7 @@ __device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, cons
   const unsigned before = (1u << lane) - 1;
   uint64_t tail = 0;
   int waiting = 0, at = 0;
-  each(src, [&](const float* x, int) {
+  each(src, [&](const float* x, int v) {
     uint32_t small = 0, large = 0;
 #pragma unroll
     for (int e = 0; e < S::N; ++e) {
@@ -268,22 +269,21 @@ __device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, cons
       if (!R::small(z)) large |= in ? 1u << e : 0;
       else small += in ? w : 0;
     }
-    if (__any_sync(0xffffffffu, large != 0)) {
-#pragma unroll
-      for (int e = 0; e < S::N; ++e) {
-        const bool mine = large >> e & 1;
-        const unsigned m = __ballot_sync(0xffffffffu, mine);
-        if (m == 0) continue;
-        if (mine) queue[(at + waiting + __popc(m & before)) & 63] = x[e];
-        waiting += __popc(m);
-        if (waiting < 32) continue;
-        __syncwarp();
-        const float q = queue[(at + lane) & 63];
-        __syncwarp();
-        at += 32;
-        waiting -= 32;
-        sink(q, row.large_weight(q), true);
+    // one of each lane's at a time: they are few, or every lane has all
+    while (__any_sync(0xffffffffu, large != 0)) {
+      const unsigned m = __ballot_sync(0xffffffffu, large != 0);
+      if (large) {
+        queue[(at + waiting + __popc(m & before)) & 63] = src.one(v, __ffs(large) - 1);
+        large &= large - 1;
       }
+      waiting += __popc(m);
+      if (waiting < 32) continue;
+      __syncwarp();
+      const float q = queue[(at + lane) & 63];
+      __syncwarp();
+      at += 32;
+      waiting -= 32;
+      sink(q, row.large_weight(q), true);
     }
     tail += small;
   });
@@ -358,8 +358,9 @@ struct Search {
 };
 
 // What a histogram's bins are: distances to the top, near or far, or keys.
-// Near: counts in bins of 1/16 over 32, weights in bins of 1/32 over 16 log2s;
-// far: twice as wide and long, from where the near ones end.
+// Near: counts in bins of 1/16 over 32, weights in bins of 1/28.5 over 18 log2s
+// (the large weights: all small ones are in the last bin); far: twice as wide
+// and long, from where the near ones end.
 enum Bins { kNear, kFar, kKeys };
 
 // One histogram of the tokens in `in` and [q.lo, q.hi]; q narrows to the bin
@@ -370,7 +371,7 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
                        Search& q, double p, uint64_t excess) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kFrom = BINS == kFar ? kBins / 2 : 0;
-  const float per = (WEIGHT ? row.rate_f * 32.f : 16.f) * (BINS == kFar ? 0.5f : 1.f);
+  const float per = (WEIGHT ? row.rate_f * 28.5f : 16.f) * (BINS == kFar ? 0.5f : 1.f);
   auto distance = [&](float x) {
     // (NaN, at the top where it or the rate is infinite, converts to 0)
     return max(0, min(__float2int_rz((row.top - x) * per) - kFrom, kBins - 1));
@@ -385,7 +386,7 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
     uint64_t tail = each_weight<false, false>(
         src, row, in, sh.queue[warp], nullptr,
         [&](float x, uint64_t w, bool valid) { add_warp(sh.hist, distance(x), w, valid); });
-    tail = warp_sum64(tail);  // small ones are past 18 log2s: all in the last bin
+    tail = warp_sum64(tail);
     if (lane == 0) add_parts(sh.hist, kBins - 1, tail);
   } else {
     // in the keys' range by value: -0 has a key of its own, which no token has
@@ -524,11 +525,11 @@ __device__ int collect(const Slice<T>& sl, const Cluster& cl, Shared& sh, float 
   constexpr int kHold = kWarpList;
   float* hx = sh.list_x + warp * kHold;
   int* hi = sh.list_i + warp * kHold;
-  each(sl, [&](const float* v, int i) {
+  each(sl, [&](const float* f, int v) {
     unsigned mask = 0;
 #pragma unroll
     for (int e = 0; e < Slice<T>::N; ++e)
-      if (v[e] >= x) mask |= 1u << e;
+      if (f[e] >= x) mask |= 1u << e;
     if (!__any_sync(0xffffffffu, mask != 0)) return;
     const int c = __popc(mask);
     int incl = c;
@@ -542,8 +543,8 @@ __device__ int collect(const Slice<T>& sl, const Cluster& cl, Shared& sh, float 
     for (int e = 0; e < Slice<T>::N; ++e)
       if (mask >> e & 1) {
         if (at < kHold) {
-          hx[at] = v[e];
-          hi[at] = i + e;
+          hx[at] = f[e];
+          hi[at] = sl.index(v) + e;
         }
         ++at;
       }
@@ -822,10 +823,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     // the first token of the order: the lowest index with the largest logit
     int first = 0x7fffffff;
     const float x_top = top_key == 0 ? NAN : value_of<G>(top_key);
-    each(sl, [&](const float* x, int i) {
+    each(sl, [&](const float* x, int v) {
 #pragma unroll
       for (int e = 0; e < Slice<T>::N; ++e)
-        if (x[e] == x_top) first = min(first, i + e);
+        if (x[e] == x_top) first = min(first, sl.index(v) + e);
     });
     first = __reduce_min_sync(0xffffffffu, first);
     __syncthreads();
@@ -851,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     a.logprob[r] = (float)(z - log((double)total / kOne));
   };
   // Each cut's first histogram; what lies from the first one's bin up may fit the
-  // list (far tokens are many).
+  // list.
   auto listed = [&](const Search& q, uint64_t need) {
     const int n = collect(sl, cl, sh, fmaxf(value_of<G>(q.lo), cut.x));
     if (n >= 0 && cl.rank == 0) draw_sorted(sh, row, f, n, need, write);
@@ -864,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     q.need = (uint64_t)f.k;
     const bool near = begin<false>(sl, cl, sh, row, cut, q, 0.0, 0);
     if (!q.whole) {
-      if (near && listed(q, 0)) return;
+      if (near && q.above + q.in_bin <= kList && listed(q, 0)) return;
       cut = finish<false>(sl, cl, sh, row, cut, q);
       excess = (q.in_bin - cut.ties) * row.weight(cut.x);
     }
@@ -873,7 +874,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     q = {kLowest<G>, top_key, 0, 0, q.round, false, false, 0};
     const bool near = begin<true>(sl, cl, sh, row, cut, q, f.p, excess);
     if (!q.whole) {
-      if (!by_count && near && listed(q, q.need)) return;
+      // (a bin of this width with some dozens of tokens has too many above it)
+      if (!by_count && near && q.in_bin <= 24 * row.weight(value_of<G>(q.hi)) &&
+          listed(q, q.need))
+        return;
       cut = finish<true>(sl, cl, sh, row, cut, q);
     }
   }
@@ -904,8 +908,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   draw(sl, cl, sh, row, f, cut, write);
 }
 
-// CTAs per row.  Few rows: eight, so that a row's passes are short (clusters of
-// eight are placed within a GPC, so more than 32 rows of them would queue).
+// CTAs per row.  Few rows: sixteen or eight, so that a row's passes are short (a
+// cluster is placed within a GPC, so more than 32 rows of eight would queue).
 // More rows: four; with 256 rows of 151936 logits, four take 98 us (bf16, all
 // tokens open) and 271 us (top-p 0.95), eight 121 and 314 us, one 114 and 481
 // us.  At least 2048 tokens to a CTA, at most kMaxSlice.
@@ -913,7 +917,7 @@ template <typename T>
 int launch(SampleArgs a, int64_t rows, cudaStream_t st) {
   constexpr int N = 16 / (int)sizeof(T);
   const int64_t vectors = ((int64_t)a.V + 2 * N - 2) / N;  // whatever the rows' skew
-  const int most = rows <= 32 ? 8 : 4;
+  const int most = rows <= 8 ? 16 : rows <= 32 ? 8 : 4;
   int size = 1;
   while (size < most && (int64_t)a.V >= 4096 * size) size *= 2;
   while (size < kMaxCluster && (vectors + size - 1) / size * N > kMaxSlice) size *= 2;

@@ -109,17 +109,28 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, int which, int
                  h * a.stride[which][1] + (base - start) * pitch;
   const int fresh = (int)(start > base ? start - base : 0);  // first new row
   T* tail = static_cast<T*>(a.tail[which]) + (bh * 2 + (blk & 1)) * a.block * D;
+  // a thread's vectors lie kThreads / VPR rows apart
+  const int row0 = threadIdx.x / VPR, col = threadIdx.x % VPR * 8;
+  constexpr int kApart = kThreads / VPR;
+  const bool full = live == a.block && fresh == 0;  // most blocks of a prompt
   uint4 x[NV];
+  if (full) {
+    const T* from = src + row0 * pitch + col;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = __ldcs(reinterpret_cast<const uint4*>(from + i * kApart * pitch));
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int row = row0 + i * kApart;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (row < live)
+        x[i] = *reinterpret_cast<const uint4*>(row < fresh ? tail + row * D + col
+                                                           : src + row * pitch + col);
+    }
+  }
   uint32_t top2 = 0;  // |bits| maxima of even and odd elements
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = i * kThreads + threadIdx.x;
-    const int row = v / VPR, col = (v % VPR) * 8;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (row < live) {
-      const T* from = row < fresh ? tail + row * D + col : src + row * pitch + col;
-      x[i] = *reinterpret_cast<const uint4*>(from);
-    }
     top2 = __vmaxu2(top2, x[i].x & 0x7fff7fffu);
     top2 = __vmaxu2(top2, x[i].y & 0x7fff7fffu);
     top2 = __vmaxu2(top2, x[i].z & 0x7fff7fffu);
@@ -143,23 +154,32 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, int which, int
   d.mul = qmax * down;
   d.top = amax * down;
   d.inv = __frcp_rn(d.top);
-  uint8_t* codes = a.codes[which] + (bh * a.max_len + base) * D;
-  auto store = [&](auto&& quantise) {
+  uint8_t* codes = a.codes[which] + (bh * a.max_len + base + row0) * D + col;
+  if (full && finite && d.top >= 1e-20f) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      *reinterpret_cast<uint2*>(codes + i * kApart * D) = quantise8<T, FMT, false>(x[i], d);
+  } else {
+    const bool tiny = d.top < 1e-20f;  // so small that remainders would be rounded
+#pragma unroll 1
+    for (int i = 0; i < NV; ++i) {
+      if (row0 + i * kApart >= live) break;
+      uint4 y = x[0];
+#pragma unroll
+      for (int j = 1; j < NV; ++j)
+        if (j == i) y = x[j];
+      uint2 q = make_uint2(0, 0);
+      if (finite) q = tiny ? quantise8<T, FMT, true>(y, d) : quantise8<T, FMT, false>(y, d);
+      *reinterpret_cast<uint2*>(codes + i * kApart * D) = q;
+    }
+  }
+  if (keep) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = i * kThreads + threadIdx.x;
-      const int row = v / VPR, col = (v % VPR) * 8;
-      if (row >= live) continue;
-      *reinterpret_cast<uint2*>(codes + row * D + col) = quantise(x[i]);
-      if (keep && row >= fresh) *reinterpret_cast<uint4*>(tail + row * D + col) = x[i];
+      const int row = row0 + i * kApart;
+      if (row >= fresh && row < live) *reinterpret_cast<uint4*>(tail + row * D + col) = x[i];
     }
-  };
-  if (!finite)
-    store([](const uint4&) { return make_uint2(0, 0); });
-  else if (d.top < 1e-20f)  // so small that remainders would be rounded
-    store([&](const uint4& y) { return quantise8<T, FMT, true>(y, d); });
-  else
-    store([&](const uint4& y) { return quantise8<T, FMT, false>(y, d); });
+  }
 }
 
 // Grid ({K, V} x kv heads, blocks a call can touch, batch): heads next to one

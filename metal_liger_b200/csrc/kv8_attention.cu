@@ -35,6 +35,7 @@
 #include "kv8.cuh"
 
 #include <cuda_fp8.h>
+#include <type_traits>
 
 namespace ml {
 namespace {
@@ -53,7 +54,7 @@ struct AttnArgs {
   void* out;                // [B, T, Hq, D]
   float* part;              // [2 * gridDim.x] pieces; null: a CTA per segment
   int ctas;                 // CTAs that share the flat list
-  bool split;               // the join: several CTAs to a segment
+  int split;                // the join: CTAs of a segment
 };
 
 // A segment counts as this many tiles more than it has when the list is cut
@@ -873,26 +874,24 @@ kv8_attention_kernel(const __grid_constant__ AttnArgs a) {
   }
 }
 
-// Joins the segments that cross CTAs.  The pieces' statistics become one factor
-// per piece and row (a row per warp, lanes over the pieces).  Few segments have
-// many pieces: a CTA takes 32 items of one, a warp every kJoinGroups-th piece,
-// so that few loads follow one another, and the warps' sums are added in
-// order.  Many segments have few: a CTA takes one, a warp 32 items of all its
-// pieces.
+// Joins the segments that cross CTAs, `split` CTAs each.  The pieces' statistics
+// become one factor per piece and row (a row per warp, lanes over the pieces);
+// then the threads take the CTA's items (four values of every piece), in groups
+// where there are fewer items than threads: a group takes every group-count-th
+// piece, so that few loads follow one another, and the groups' sums are added in
+// order.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinGroups = kJoinThreads / 32;
 constexpr int kMaxCtas = 640;  // of the list
 
 template <typename T, int D, int NT, int NW>
 __global__ void __launch_bounds__(kJoinThreads)
 kv8_attention_join(const __grid_constant__ AttnArgs a) {
   using C = Config<D, NT, NW>;
-  constexpr int kParts = C::kImage / 4 / 32;  // of 32 items
   __shared__ __align__(8) float factor[kMaxCtas][C::kRows];
-  __shared__ float4 sums[kJoinGroups][32];
+  __shared__ float4 sums[kJoinThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per_b = a.kv_heads * a.row_tiles;
-  const int segment = a.split ? blockIdx.x / kParts : blockIdx.x;
+  const int segment = blockIdx.x / a.split;
   const int b = segment / per_b, seg = segment % per_b;
   // start and counts may be read before the wait: this grid starts when the
   // first kernel's CTAs have passed theirs, and that kernel writes neither
@@ -916,6 +915,7 @@ kv8_attention_join(const __grid_constant__ AttnArgs a) {
   auto piece = [&](int i) -> const float* {
     return a.part + ((int64_t)(c0 + i) * C::kCtaPieces + (i == 0 ? 1 : 0)) * C::kPiece;
   };
+#pragma unroll
   for (int r = warp; r < C::kRows; r += kJoinThreads / 32) {
     const bool sees = rt * C::kRows + r < a.rows && visible(a, b, (rt * C::kRows + r) / a.group) > 0;
     float M = -INFINITY, MO = -INFINITY, L = 0.f;
@@ -948,28 +948,33 @@ kv8_attention_join(const __grid_constant__ AttnArgs a) {
     }
   }
   __syncthreads();
-  float o[4];
-  if (!a.split) {
-    for (int x = threadIdx.x; x < kParts * 32; x += kJoinThreads) {
-      sum_item<D, NT, 1>(x, 0, count, piece, factor, o);
-      write_item<T, D, NT>(a, b, seg, x, o);
-    }
-    return;
-  }
-  const int item = blockIdx.x % kParts * 32 + lane;
-  sum_item<D, NT, kJoinGroups>(item, warp, count, piece, factor, o);
-  sums[warp][lane] = make_float4(o[0], o[1], o[2], o[3]);
-  __syncthreads();
-  if (warp > 0) return;
+  const int items = C::kImage / 4 / a.split, first = (int)(blockIdx.x % a.split) * items;
+  auto join = [&](auto groups) {
+    constexpr int G = decltype(groups)::value;
+    const int group = threadIdx.x / (kJoinThreads / G);
+    for (int x = threadIdx.x % (kJoinThreads / G); x < items; x += kJoinThreads) {
+      float o[4];
+      sum_item<D, NT, G>(first + x, group, count, piece, factor, o);
+      if constexpr (G > 1) {  // items = kJoinThreads / G: one round
+        sums[threadIdx.x] = make_float4(o[0], o[1], o[2], o[3]);
+        __syncthreads();
+        if (group > 0) return;
 #pragma unroll
-  for (int i = 1; i < kJoinGroups; ++i) {
-    const float4 x = sums[i][lane];
-    o[0] += x.x;
-    o[1] += x.y;
-    o[2] += x.z;
-    o[3] += x.w;
-  }
-  write_item<T, D, NT>(a, b, seg, item, o);
+        for (int i = 1; i < G; ++i) {
+          const float4 y = sums[i * (kJoinThreads / G) + x];
+          o[0] += y.x;
+          o[1] += y.y;
+          o[2] += y.z;
+          o[3] += y.w;
+        }
+      }
+      write_item<T, D, NT>(a, b, seg, first + x, o);
+    }
+  };
+  if (items >= kJoinThreads) join(std::integral_constant<int, 1>());
+  else if (items == kJoinThreads / 2) join(std::integral_constant<int, 2>());
+  else if (items == kJoinThreads / 4) join(std::integral_constant<int, 4>());
+  else join(std::integral_constant<int, 8>());  // 32: the least that the host's rule gives
 }
 
 // Query rows per tile: 8 NT.
@@ -1029,11 +1034,14 @@ int launch(AttnArgs a, cudaStream_t st) {
   constexpr int NW = list_warps(D, NT);
   const int rc = launch_kernel<T, FMT, D, NT, NW>(a, a.ctas, st);
   if (rc != ML_OK) return rc;
-  const int64_t parts = Config<D, NT, NW>::kImage / 4 / 32;
-  a.split = segs * parts <= 4 * num_sms();
-  ML_CHECK_CUDA(launch_pdl(kv8_attention_join<T, D, NT, NW>,
-                           dim3((unsigned)(a.split ? segs * parts : segs)), dim3(kJoinThreads), 0,
-                           st, a),
+  // as many CTAs as four to an SM, each with 32 items or more.  Against all or
+  // nothing (32 items a CTA, or a CTA to a segment): 32 segments of 4000 positions
+  // 23.5 for 27 us, 8 of 65536 34.9 for 34.6, 20 of 777 13.2 for 12.7
+  a.split = 1;
+  while (a.split * 2 <= Config<D, NT, NW>::kImage / 4 / 32 && segs * a.split * 2 <= 4 * num_sms())
+    a.split *= 2;
+  ML_CHECK_CUDA(launch_pdl(kv8_attention_join<T, D, NT, NW>, dim3((unsigned)(segs * a.split)),
+                           dim3(kJoinThreads), 0, st, a),
                 "kv8_attention(join)");
   return ML_OK;
 }

@@ -252,6 +252,11 @@ _KV8_ATTN = "metal_liger_kv8"
 _KV8_CACHE: list = [None]
 
 
+def _windowed(window: Optional[int], cache) -> bool:
+    """Whether a sliding window hides any position of the cache."""
+    return window is not None and window < cache.max_seq_len
+
+
 def _kv8_attention_forward(module, query, key, value, attention_mask, dropout=0.0, scaling=None,
                            **kwargs):
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
@@ -262,6 +267,12 @@ def _kv8_attention_forward(module, query, key, value, attention_mask, dropout=0.
         return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
                                       scaling=scaling, **kwargs)
     cache.pending.discard(layer)
+    extra = [n for n in ("softcap", "s_aux") if kwargs.get(n) is not None]
+    if _windowed(kwargs.get("sliding_window"), cache):
+        extra.append("sliding_window")
+    if extra:
+        raise RuntimeError(f"kv_cache_dtype: the decoder's attention has {', '.join(extra)}, which "
+                           "the attention over the 8-bit cache does not")
     scale = float(scaling) if scaling is not None else query.shape[-1] ** -0.5
     return cache.decode_attention(layer, query, scale), None
 
@@ -457,6 +468,9 @@ def _decode_block_ok(attn, cache) -> bool:
     if cache.head_dim != D or attn.q_proj.out_features % D or attn.k_proj.out_features != \
             cache.num_kv_heads * D or attn.v_proj.out_features != cache.num_kv_heads * D:
         return False
+    if isinstance(cache, MetalLigerQuantizedCache) and _windowed(
+            getattr(attn, "sliding_window", None), cache):
+        return False  # refused by the attention itself
     G = attn.q_proj.out_features // D // cache.num_kv_heads
     return (G * cache.num_kv_heads * D == attn.q_proj.out_features and G in (1, 2, 4, 8, 16)
             and G * D <= 1024)
@@ -869,7 +883,9 @@ class MetalLigerGenerator:
         full static buffers under a mask).
 
         The keyword-only arguments are not in the reference either.
-        ``kv_cache_dtype`` "int8" or "fp8" holds the KV cache in 8 bits.
+        ``kv_cache_dtype`` "int8" or "fp8" holds the KV cache in 8 bits; decode
+        steps then attend to every position before them, so a mask that hides
+        some (padding) and sliding windows are refused.
         ``fused_sampling`` (implied by ``top_k`` or ``min_p``) draws every token,
         the first included, with ``ops.fused_sampling`` from ``temperature``,
         ``top_k``, ``top_p`` and ``min_p``, all honoured (temperature 0 is
@@ -877,6 +893,11 @@ class MetalLigerGenerator:
         ``torch.Generator``) gives its uniform numbers."""
         batch_size, prompt_len = input_ids.shape
         max_len = prompt_len + max_new_tokens
+        if kv_cache_dtype is not None:
+            seen = kwargs.get("attention_mask")
+            if seen is not None and (seen.dim() != 2 or not bool((seen != 0).all())):
+                raise ValueError("generate: kv_cache_dtype takes no padded batch and no attention "
+                                 "mask of its own")
         fused = (fused_sampling or top_k is not None or min_p is not None) and temperature != 0
         greedy = not fused and (temperature == 0 or (temperature == 1.0 and top_p == 1.0))
         if cuda_graph is None:
@@ -887,7 +908,7 @@ class MetalLigerGenerator:
             sampling = {"temperature": float(temperature), "top_k": int(top_k or 0),
                         "top_p": float(top_p), "min_p": float(min_p or 0.0)}
             _check_sampling(**sampling)
-            uniform = torch.rand((max_new_tokens, batch_size), generator=generator,
+            uniform = torch.rand((max(max_new_tokens, 1), batch_size), generator=generator,
                                  device=input_ids.device)
         static = (greedy or fused) and not kwargs and cuda_graph and max_new_tokens > 1
         if static:

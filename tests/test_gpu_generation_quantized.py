@@ -166,3 +166,14 @@ def test_eos_stops_and_refusals():
         with _QuantizedAttention(m2.model, cache):
             cache.update(k, k, 1)
     assert m2.model.config._attn_implementation == "sdpa"
+
+
+@pytest.mark.parametrize("new", [0, 1])
+def test_fused_sampling_of_no_and_one_token(new):
+    g = MetalLigerGenerator(_model(seed=12))
+    ids = _ids(2, 6)
+    out = g.generate(ids, max_new_tokens=new, kv_cache_dtype="int8", top_k=1)
+    assert torch.equal(out, g.generate(ids, max_new_tokens=new))
+    padded = torch.ones_like(ids)
+    assert torch.equal(out, g.generate(ids, max_new_tokens=new, kv_cache_dtype="int8", top_k=1,
+                                       attention_mask=padded))

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from metal_liger_b200 import _C
+from metal_liger_b200 import _C, generation
 from metal_liger_b200.ops.fused_sampling import fused_sample
 from metal_liger_b200.ops.quantized_kv import (
     allocate_quantized_kv, quantized_kv_append, quantized_kv_attention)
@@ -136,3 +136,36 @@ def test_oracle_sampler_on_known_rows():
     assert OD.sample_row(x, 0.5, 1.0, 0, 0.5, 0.0)[2] == [1, 3]
     assert OD.sample_row(x, 0.5, 1.0, 0, 1.0, 0.45)[2] == [1, 2, 3]
     assert OD.sample_row(x, 0.5, 0.0, 0, 1.0, 0.0)[:2] == (1, 0.0)
+
+
+def test_generate_refuses_hidden_positions():
+    g = generation.MetalLigerGenerator.__new__(generation.MetalLigerGenerator)
+    ids = torch.zeros(2, 4, dtype=torch.int64)
+    padded = torch.tensor([[0, 1, 1, 1], [1, 1, 1, 1]])
+    for mask in (padded, torch.zeros(2, 1, 4, 4)):
+        with pytest.raises(ValueError, match="mask"):
+            g.generate(ids, kv_cache_dtype="int8", attention_mask=mask)
+
+
+@pytest.mark.parametrize("extra,refused", [
+    (dict(sliding_window=31), True), (dict(softcap=30.0), True), (dict(s_aux=torch.zeros(2)), True),
+    (dict(sliding_window=32, softcap=None), False), (dict(sliding_window=None), False)])
+def test_attention_over_the_codes_refuses_what_it_lacks(monkeypatch, extra, refused):
+    class Cache:
+        pending, max_seq_len = {3}, 32
+
+        def decode_attention(self, layer, query, scale):
+            return layer, scale
+
+    class Module:
+        layer_idx = 3
+
+    monkeypatch.setattr(generation, "_KV8_CACHE", [Cache()])
+    q = torch.zeros(1, 2, 1, 64)
+    if refused:
+        with pytest.raises(RuntimeError, match=next(iter(extra))):
+            generation._kv8_attention_forward(Module(), q, q, q, None, scaling=0.5, **extra)
+    else:
+        Cache.pending = {3}
+        out, _ = generation._kv8_attention_forward(Module(), q, q, q, None, scaling=0.5, **extra)
+        assert out == (3, 0.5)

@@ -17,8 +17,9 @@
 // summed as integers: W = round(2^43 w), which keeps V <= 2^20 of them below
 // 2^63 and is exact in any order.  Where w < 2^-18 it comes from the fp32
 // exponential, with what rounding took from its argument put back (off by
-// 2^-22 of it, so by 2^-40 of the largest at most), above from fp64: 2^(i/256) from a table times a quartic in the rest, |r| <=
-// 2^-9, good to 2^-50.
+// 2^-22 of it, so by 2^-40 of the largest at most); above from fp64:
+// 2^(i/64) from a table times Taylor's quintic in the rest, |r| <= 2^-7, whose
+// first term left out is below 2^-54.
 //
 // A cluster of CTAs holds a row in shared memory, so HBM is read once; every
 // step is then a pass over the CTA's slice and an exchange of a few words

@@ -248,16 +248,50 @@ __device__ __forceinline__ void each(const S& src, F&& f) {
   }
 }
 
+// Tokens that few lanes have, handed on a warp at a time.
+struct Queue {
+  float* held;  // 64
+  int at = 0, waiting = 0;
+
+  // `mask`: of the tokens of vector v, this lane's; sink(x, valid).
+  template <typename S, typename F>
+  __device__ __forceinline__ void push(const S& src, int v, uint32_t mask, F&& sink) {
+    const int lane = threadIdx.x & 31;
+    // one of each lane's at a time: they are few, or every lane has all
+    while (__any_sync(0xffffffffu, mask != 0)) {
+      const unsigned m = __ballot_sync(0xffffffffu, mask != 0);
+      if (mask) {
+        held[(at + waiting + __popc(m & ((1u << lane) - 1))) & 63] = src.one(v, __ffs(mask) - 1);
+        mask &= mask - 1;
+      }
+      waiting += __popc(m);
+      if (waiting < 32) continue;
+      __syncwarp();
+      const float q = held[(at + lane) & 63];
+      __syncwarp();
+      at += 32;
+      waiting -= 32;
+      sink(q, true);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void flush(float none, F&& sink) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    if (waiting) sink(lane < waiting ? held[(at + lane) & 63] : none, lane < waiting);
+    __syncwarp();
+  }
+};
+
 // each() for weights: sink(x, W, valid) gets the large ones, a warp at a time;
 // the sum of this lane's small ones is returned.  OPEN: the cut has everything.
 // TIES: this lane's tokens equal to the cut's x are counted.
 template <bool OPEN, bool TIES, typename S, typename R, typename F>
 __device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, const Cut& cut,
                                                 float* queue, int* ties, F&& sink) {
-  const int lane = threadIdx.x & 31;
-  const unsigned before = (1u << lane) - 1;
   uint64_t tail = 0;
-  int waiting = 0, at = 0;
+  Queue waiting = {queue};
+  auto weigh = [&](float x, bool valid) { sink(x, row.large_weight(x), valid); };
   each(src, [&](const float* x, int v) {
     uint32_t small = 0, large = 0;
 #pragma unroll
@@ -270,30 +304,10 @@ __device__ __forceinline__ uint64_t each_weight(const S& src, const R& row, cons
       if (!R::small(z)) large |= in ? 1u << e : 0;
       else small += in ? w : 0;
     }
-    // one of each lane's at a time: they are few, or every lane has all
-    while (__any_sync(0xffffffffu, large != 0)) {
-      const unsigned m = __ballot_sync(0xffffffffu, large != 0);
-      if (large) {
-        queue[(at + waiting + __popc(m & before)) & 63] = src.one(v, __ffs(large) - 1);
-        large &= large - 1;
-      }
-      waiting += __popc(m);
-      if (waiting < 32) continue;
-      __syncwarp();
-      const float q = queue[(at + lane) & 63];
-      __syncwarp();
-      at += 32;
-      waiting -= 32;
-      sink(q, row.large_weight(q), true);
-    }
+    waiting.push(src, v, large, weigh);
     tail += small;
   });
-  __syncwarp();
-  if (waiting) {
-    const float q = lane < waiting ? queue[(at + lane) & 63] : row.top;
-    sink(q, row.large_weight(q), lane < waiting);
-  }
-  __syncwarp();
+  waiting.flush(row.top, weigh);
   return tail;
 }
 
@@ -394,16 +408,24 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
     constexpr uint32_t kMinusZero = 0x7fffffffu >> R::kKey;
     const float x_lo = fmaxf(value_of<R::kKey>(q.lo == kMinusZero ? q.lo + 1 : q.lo), in.x);
     const float x_hi = value_of<R::kKey>(q.hi == kMinusZero ? q.hi - 1 : q.hi);
-    each(src, [&](const float* x, int) {
+    auto bin_of = [&](float x) {
+      return BINS == kKeys ? (int)((q.hi - key_of<R::kKey>(x)) >> shift) : distance(x);
+    };
+    Queue some = {sh.queue[warp]};
+    auto weigh = [&](float x, bool valid) {
+      if (valid) add_parts(sh.hist, bin_of(x), row.weight(x));
+    };
+    each(src, [&](const float* x, int v) {
+      uint32_t mask = 0;
 #pragma unroll
       for (int e = 0; e < S::N; ++e) {
-        if (!(x[e] >= x_lo && x[e] <= x_hi)) continue;
-        const int bin =
-            BINS == kKeys ? (int)((q.hi - key_of<R::kKey>(x[e])) >> shift) : distance(x[e]);
-        if (WEIGHT) add_parts(sh.hist, bin, row.weight(x[e]));
-        else atomicAdd(&sh.hist[0][bin], 1u);
+        const bool in_range = x[e] >= x_lo && x[e] <= x_hi;
+        if (WEIGHT) mask |= in_range ? 1u << e : 0;
+        else if (in_range) atomicAdd(&sh.hist[0][bin_of(x[e])], 1u);
       }
+      if (WEIGHT) some.push(src, v, mask, weigh);
     });
+    if (WEIGHT) some.flush(row.top, weigh);
   }
   __syncthreads();
   uint64_t s = sh.hist[0][tid] + ((uint64_t)sh.hist[1][tid] << 15) + ((uint64_t)sh.hist[2][tid] << 30);
@@ -493,14 +515,28 @@ __device__ void narrow(const S& src, const Cluster& cl, Shared& sh, const R& row
   q.hi = sh.key[1] - 1;
 }
 
-// The histograms by distance; false where they go past the near ones.
-template <bool WEIGHT, typename S, typename R>
-__device__ bool begin(const S& src, const Cluster& cl, Shared& sh, const R& row, const Cut& in,
-                      Search& q, double p, uint64_t excess) {
-  narrow<WEIGHT, kNear>(src, cl, sh, row, in, q, p, excess);
-  if (q.whole || !q.beyond) return true;
-  narrow<WEIGHT, kFar>(src, cl, sh, row, in, q, p, excess);
-  return false;
+// The key of the smallest logit that min-p keeps, by 32-way search.
+template <int G>
+__device__ uint32_t least_key(Shared& sh, const Row<G>& row, float least, uint32_t top_key) {
+  const int lane = threadIdx.x & 31;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    uint32_t lo = kLowest<G>, hi = top_key;  // the answer lies in [lo, hi]: the largest qualifies
+    while (lo < hi) {
+      const uint32_t step = (hi - lo + 31) / 32;
+      const uint64_t k = (uint64_t)lo + (uint64_t)step * lane;
+      const bool ok = k >= hi || row.exact(value_of<G>((uint32_t)k)) >= (double)least;
+      const unsigned m = __ballot_sync(0xffffffffu, ok);
+      const int j = m ? __ffs(m) - 1 : 32;
+      const uint64_t top_k = (uint64_t)lo + (uint64_t)step * j;
+      const uint32_t nh = top_k < hi ? (uint32_t)top_k : hi;
+      lo = j == 0 ? nh : (uint32_t)((uint64_t)lo + (uint64_t)step * (j - 1) + 1);
+      hi = nh;
+    }
+    if (lane == 0) sh.key[0] = lo;
+  }
+  __syncthreads();
+  return sh.key[0];
 }
 
 // Narrows to one key; as many of the tokens equal to it are left as still needed.
@@ -670,8 +706,6 @@ __device__ void draw_sorted(Shared& sh, const R& row, const Filter& f, int n, ui
   if (run > target && run - w <= target) write(sh.list_i[tid], total);
 }
 
-// Cuts and draws from `src`, whose tokens are in `in`; `q` is the selection that
-// has begun on the first of the two cuts that are on.  first: top index.
 // Draws from the slices' tokens in `cut`.
 template <typename S, typename R, typename W>
 __device__ void draw(const S& src, const Cluster& cl, Shared& sh, const R& row, const Filter& f,
@@ -854,57 +888,59 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   };
   // Each cut's first histogram; what lies from the first one's bin up may fit the
   // list.
-  auto listed = [&](const Search& q, uint64_t need) {
-    const int n = collect(sl, cl, sh, fmaxf(value_of<G>(q.lo), cut.x));
+  auto listed = [&](float x, uint64_t need) {
+    const int n = collect(sl, cl, sh, fmaxf(x, cut.x));
     if (n >= 0 && cl.rank == 0) draw_sorted(sh, row, f, n, need, write);
     return n >= 0;  // nothing of the other CTAs is needed any more
+  };
+  float x_least = Cut::kNone;  // of min-p; once it is known:
+  auto cut_least = [&] {
+    if (!(x_least > cut.x)) return;
+    cut.x = x_least;
+    cut.ties = ~(uint64_t)0;
   };
   Search q = {kLowest<G>, top_key, 0, 0, 0, false, false, 0};
   const bool by_count = f.k > 0 && f.k < a.V;
   uint64_t excess = 0;
   if (by_count) {
     q.need = (uint64_t)f.k;
-    const bool near = begin<false>(sl, cl, sh, row, cut, q, 0.0, 0);
+    narrow<false, kNear>(sl, cl, sh, row, cut, q, 0.0, 0);
     if (!q.whole) {
-      if (near && q.above + q.in_bin <= kList && listed(q, 0)) return;
+      const bool near = !q.beyond;
+      if (near && q.above + q.in_bin <= kList && listed(value_of<G>(q.lo), 0)) return;
+      if (!near) narrow<false, kFar>(sl, cl, sh, row, cut, q, 0.0, 0);
       cut = finish<false>(sl, cl, sh, row, cut, q);
       excess = (q.in_bin - cut.ties) * row.weight(cut.x);
     }
   }
   if (f.p < 1.0) {
     q = {kLowest<G>, top_key, 0, 0, q.round, false, false, 0};
-    const bool near = begin<true>(sl, cl, sh, row, cut, q, f.p, excess);
+    narrow<true, kNear>(sl, cl, sh, row, cut, q, f.p, excess);
     if (!q.whole) {
-      // (a bin of this width with some dozens of tokens has too many above it)
-      if (!by_count && near && q.in_bin <= 24 * row.weight(value_of<G>(q.hi)) &&
-          listed(q, q.need))
-        return;
-      cut = finish<true>(sl, cl, sh, row, cut, q);
+      const bool near = !q.beyond;
+      uint32_t least = 0;
+      if (f.least > 0.f) {
+        least = least_key<G>(sh, row, f.least, top_key);
+        x_least = value_of<G>(least);
+      }
+      if (least > q.hi) {  // min-p ends before the bin that top-p ends in
+        cut_least();
+        if (!by_count && q.above <= (uint64_t)(kList * kOne * (double)f.least) &&
+            listed(cut.x, q.need))
+          return;
+      } else {
+        // (a bin of this width with some dozens of tokens has too many above it)
+        if (!by_count && near && q.in_bin <= 24 * row.weight(value_of<G>(q.hi)) &&
+            listed(value_of<G>(q.lo), q.need))
+          return;
+        if (!near) narrow<true, kFar>(sl, cl, sh, row, cut, q, f.p, excess);
+        cut = finish<true>(sl, cl, sh, row, cut, q);
+      }
     }
   }
-  // min-p: the smallest logit whose weight is large enough, by 32-way search
   if (f.least > 0.f) {
-    if (warp == 0) {
-      uint32_t lo = kLowest<G>, hi = top_key;  // the answer lies in [lo, hi]: the largest qualifies
-      while (lo < hi) {
-        const uint32_t step = (hi - lo + 31) / 32;
-        const uint64_t k = (uint64_t)lo + (uint64_t)step * lane;
-        const bool ok = k >= hi || row.exact(value_of<G>((uint32_t)k)) >= (double)f.least;
-        const unsigned m = __ballot_sync(0xffffffffu, ok);
-        const int j = m ? __ffs(m) - 1 : 32;
-        const uint64_t top_k = (uint64_t)lo + (uint64_t)step * j;
-        const uint32_t nh = top_k < hi ? (uint32_t)top_k : hi;
-        lo = j == 0 ? nh : (uint32_t)((uint64_t)lo + (uint64_t)step * (j - 1) + 1);
-        hi = nh;
-      }
-      if (lane == 0) sh.key[0] = lo;
-    }
-    __syncthreads();
-    const float x = value_of<G>(sh.key[0]);
-    if (x > cut.x) {
-      cut.x = x;
-      cut.ties = ~(uint64_t)0;
-    }
+    if (x_least == Cut::kNone) x_least = value_of<G>(least_key<G>(sh, row, f.least, top_key));
+    cut_least();
   }
   draw(sl, cl, sh, row, f, cut, write);
 }

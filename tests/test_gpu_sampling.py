@@ -73,6 +73,25 @@ def test_flat_logits_wide_nucleus(dtype):
     _check(x, u, temperature=0.05, top_p=0.99)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("spread", [0.05, 1.0, 2.5, 12.0])
+@pytest.mark.parametrize("top_k", [0, 3000])
+def test_min_p_around_the_end_of_top_p(dtype, spread, top_k):
+    """min-p ends at, just before, just after and far from the token that top-p
+    ends at."""
+    gen = torch.Generator().manual_seed(int(spread * 100) + top_k)
+    x = _logits(gen, 1, 20011, dtype, spread)
+    top_p = 0.9
+    _, _, kept = OD.sample_row(x[0], 0.5, 1.0, top_k, float(torch.tensor(top_p)), 0.0)
+    w = (x[0].double() - x[0].max().double()).exp()
+    end = w[torch.as_tensor(list(kept))].min().item()
+    least = torch.tensor([end * f for f in (1e-3, 0.5, 0.97, 0.999, 1.001, 1.03, 2.0, 30.0)])
+    least = least.clamp(max=0.999)
+    n = least.numel()
+    u = torch.rand(n, generator=gen)
+    _check(x.expand(n, -1).contiguous(), u, top_p=top_p, top_k=top_k, min_p=least)
+
+
 def test_equal_logits_keep_the_lowest_indices():
     x = torch.full((4, 1000), 2.5)
     u = torch.tensor([0.0, 0.25, 0.5, 0.999])

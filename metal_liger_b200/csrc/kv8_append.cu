@@ -24,6 +24,12 @@
 // block-wide maximum of |bits| (for bf16 and fp16 the order of the magnitudes
 // with inf and NaN on top), then the codes.  Rows past the last new one are
 // left as they were.  Memory bound: 2 bytes read and 1 written per element.
+//
+// Measured: 8 prompts of 4096 rows, 8 heads of dim 128 (205 MB) 41.5 us, 4.9
+// TB/s (60 us where blocks of new rows had row checks as well, 75 us with 512
+// threads, 64 with 128); one row for each of 64 sequences 8.2 us: two loads that
+// follow one another (start, then the rows, the tail's from L2) and a launch
+// (7.0 with 128 threads, which the prompts pay for).
 #include "kv8.cuh"
 
 #include <cuda_fp8.h>

@@ -59,7 +59,8 @@ struct AttnArgs {
 
 // A segment counts as this many tiles more than it has when the list is cut
 // into equal runs: reading its queries and writing its rows take a warp about
-// as long as one or two tiles.
+// as long as one or two tiles (2 against 0: 32 segments of 8000 positions 21.1
+// us / 22.3, 8 of 65000 33.7 / 34.9).
 constexpr int kPad = 2;
 
 // NW warps, each with a ring of units of 32 positions of K or of V.
@@ -78,7 +79,7 @@ struct Config {
 // Warps of a CTA of the list (two CTAs to an SM) ...
 constexpr int list_warps(int D, int NT) { return D * NT >= 256 ? 4 : 8; }
 // ... and of a CTA that has a segment to itself.
-constexpr int segment_warps(int D, int NT) { return 2 * list_warps(D, NT); }
+constexpr int segment_warps(int D) { return 2 * list_warps(D, 1); }
 
 // ---------------------------------------------------------------------------
 // The flat list of tiles
@@ -977,36 +978,39 @@ kv8_attention_join(const __grid_constant__ AttnArgs a) {
   else join(std::integral_constant<int, 8>());  // 32: the least that the host's rule gives
 }
 
-// Query rows per tile: 8 NT.
-inline int n_tiles(int64_t rows, int64_t dim) { return rows > 8 && dim != 256 ? 2 : 1; }
-
-// Caches this short go a CTA to a segment, in one launch.
-constexpr int64_t kOneLaunchLen = 512;
-
-inline bool one_launch(const ml_kv8_cache* c) { return c->max_len <= kOneLaunchLen; }
-
-// CTAs of the list: two waves of two per SM, which even out what one wave
-// leaves (CTAs with equal runs differ by up to a quarter in time), one where
-// there is too little work for that.
-inline int ctas_of_list(const ml_kv8_cache* c, int64_t row_tiles, int warps) {
-  const int one = 2 * num_sms();
-  const int64_t most = c->batch * c->kv_heads * row_tiles * (c->max_len / kTile + kPad);
-  const int ctas = most >= (int64_t)one * warps * 16 ? 2 * one : one;
-  return ctas < kMaxCtas ? ctas : kMaxCtas;
+// Query rows per tile: 8 NT.  Sixteen rows read the codes once instead of twice,
+// eight leave room for twice the warps, which gives more where a warp has few
+// tiles.  Eight against sixteen, 16 rows a kv head of dim 128: 4 x 8 heads of
+// 1500 positions (3000 tiles of eight rows) 15.3 us / 17.8, 4 x 8 of 8000 (16000)
+// 28.8 / 29.7, 16 x 8 of 8000 (64000) 87 / 78; dim 64, 16 x 8 of 8000 60 / 48.
+inline int n_tiles(const ml_kv8_cache* c, int64_t rows) {
+  const int64_t tiles = c->batch * c->kv_heads * ((rows + 7) / 8) * (c->max_len / kTile);
+  return rows > 8 && c->head_dim != 256 && tiles >= 128 * (int64_t)num_sms() ? 2 : 1;
 }
+
+// Short caches go a CTA to a segment, in one launch, where these are one wave
+// (one such CTA fills an SM).  One launch against the list, 64 segments: 250
+// positions 7.3 us / 13.1, 1000 11.6 / 13.7, 2000 16.1 / 16.1; 8 segments: 1000
+// 11.4 / 10.9, 2000 15.7 / 11.4; 256 segments: 250 14.5 / 14.5, 500 17.8 / 16.6.
+constexpr int64_t kOneLaunchLen = 1024;
 
 struct Plan {
   int nt, row_tiles, ctas;
-  size_t workspace;
+  size_t workspace;  // 0: one launch
 };
 inline Plan plan_of(const ml_kv8_cache* c, int64_t rows) {
   Plan p;
-  p.nt = n_tiles(rows, c->head_dim);
+  p.nt = n_tiles(c, rows);
   p.row_tiles = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+  p.ctas = 2 * num_sms() < kMaxCtas ? 2 * num_sms() : kMaxCtas;
+  const int64_t segs = c->batch * c->kv_heads * p.row_tiles;
+  if (p.nt == 1 && c->max_len <= kOneLaunchLen && segs <= num_sms()) {
+    p.workspace = 0;
+    return p;
+  }
   const int warps = list_warps((int)c->head_dim, p.nt);
-  p.ctas = ctas_of_list(c, p.row_tiles, warps);
   const int64_t piece = p.nt * c->head_dim / 16 * 4 * 32 + 3 * 8 * p.nt;
-  p.workspace = one_launch(c) ? 0 : (size_t)p.ctas * (2 + warps) * piece * sizeof(float);
+  p.workspace = (size_t)p.ctas * (2 + warps) * piece * sizeof(float);
   return p;
 }
 
@@ -1029,14 +1033,15 @@ int launch(AttnArgs a, cudaStream_t st) {
   const int64_t segs = (int64_t)a.batch * a.kv_heads * a.row_tiles;
   ML_CHECK_ARG(segs * (a.max_len / kTile + kPad) < ((int64_t)1 << 31),
                "kv8_attention: too many query rows for this cache in one call");
-  if (a.part == nullptr)
-    return launch_kernel<T, FMT, D, NT, segment_warps(D, NT)>(a, segs, st);
+  if constexpr (NT == 1) {
+    if (a.part == nullptr) return launch_kernel<T, FMT, D, 1, segment_warps(D)>(a, segs, st);
+  }
   constexpr int NW = list_warps(D, NT);
   const int rc = launch_kernel<T, FMT, D, NT, NW>(a, a.ctas, st);
   if (rc != ML_OK) return rc;
   // as many CTAs as four to an SM, each with 32 items or more.  Against all or
-  // nothing (32 items a CTA, or a CTA to a segment): 32 segments of 4000 positions
-  // 23.5 for 27 us, 8 of 65536 34.9 for 34.6, 20 of 777 13.2 for 12.7
+  // nothing (32 items a CTA, or a CTA to a segment): 64 segments of 4000 positions
+  // 23.5 for 27 us, 8 of 65536 34.9 for 34.6
   a.split = 1;
   while (a.split * 2 <= Config<D, NT, NW>::kImage / 4 / 32 && segs * a.split * 2 <= 4 * num_sms())
     a.split *= 2;

@@ -34,6 +34,11 @@
 //
 // Tokens that need fp64 are rare in most rows and everywhere in flat ones: a
 // warp queues them and weighs 32 at a time.
+//
+// Bound by instructions and by the steps that follow one another, not by
+// memory.  Measured, 151936 tokens: one row, top-k and top-p, 15 us; 64 rows, top-p
+// and min-p, 53 us (without the list 96, with top-p's end always searched for
+// 68); 256 fp32 rows with nothing cut 105 us (1.5 TB/s).
 #include "common.cuh"
 
 #include <cooperative_groups.h>

@@ -205,6 +205,27 @@ def test_attention_against_the_definition(fmt, B, Hq, Hkv, L, D, block, T, dtype
     _check_attention(kv, q, starts, counts)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("B,Hq,Hkv,L,D,block,T,dtype,starts,counts", [
+    # more than 128 tiles of eight rows to an SM: sixteen query rows at a time
+    (2, 16, 2, 256, 128, 64, 1251, torch.bfloat16, [-3, 200], [1251, 700]),
+    (1, 21, 3, 777, 64, 32, 300, torch.float16, [500], None),
+    (2, 32, 8, 20000, 128, 64, 3, torch.bfloat16, [19990, 12345], [3, 2]),
+    # a short cache with more segments than one wave holds, and just fewer
+    (20, 8, 8, 300, 128, 64, 1, torch.bfloat16, [299] * 10 + [0, 1, 31, 32, 63, 64, 65, 200, -1, 298],
+     None),
+    (18, 8, 8, 1000, 64, 64, 1, torch.float16, [999], None),
+])
+def test_attention_of_many_rows_and_segments(fmt, B, Hq, Hkv, L, D, block, T, dtype, starts, counts):
+    gen = torch.Generator().manual_seed(B * 37 + Hq + L + T)
+    kv = _filled(gen, B, Hkv, L, D, block, fmt, dtype)
+    q = _rows(gen, B, Hq, T, D, dtype=dtype)
+    out = _check_attention(kv, q, starts, counts)
+    st = torch.tensor(starts, device=DEV)
+    ct = None if counts is None else torch.tensor(counts, device=DEV)
+    assert torch.equal(out, quantized_kv_attention(q.to(DEV), kv, st, ct))
+
+
 def test_attention_strided_queries_scale_and_large_scores():
     gen = torch.Generator().manual_seed(8)
     kv = _filled(gen, 2, 2, 512, 128, 64, "int8", torch.bfloat16)

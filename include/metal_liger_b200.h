@@ -712,7 +712,8 @@ ML_API int ml_kv8_append(const ml_kv8_cache* cache, const void* k, const int64_t
  * (batch, head, token), multiples of 8, head_dim contiguous; out [batch,
  * tokens, q_heads, head_dim] contiguous; both in the cache's dtype.  Rows t >=
  * counts[b], and rows that see no position, are zeros.  fp32 scores, softmax
- * statistics and accumulation.  workspace >=
+ * statistics and accumulation; the weights enter the second product in fp16.
+ * workspace >=
  * ml_kv8_attention_workspace_bytes (0: may be NULL), 16-byte aligned, not
  * shared with a call that may run at the same time.
  */

@@ -5,7 +5,7 @@
 //   scale = a / qmax,   code = round(x * qmax / a)      (qmax: 127, or 448 for e4m3)
 // rounded half to even to an integer, or to the nearest e4m3 value.  x has at
 // most 11 significant bits and qmax 7, so x * qmax is exact in fp32, the one
-// IEEE division is correctly rounded, and its quotient is a tie exactly where
+// IEEE division is correctly rounded, and it is a tie exactly where
 // the true quotient is one (two such ratios that differ do so by more than
 // 2^-22 of their size): every code is the one the formula gives in exact
 // arithmetic.  A block without a non-zero value has scale 0 and codes 0; a
@@ -23,7 +23,8 @@
 // call, older ones from the tail) go to registers as 16-byte vectors, one
 // block-wide maximum of |bits| (for bf16 and fp16 the order of the magnitudes
 // with inf and NaN on top), then the codes.  Rows past the last new one are
-// left as they were.  Memory bound: 2 bytes read and 1 written per element.
+// left as they were.  2 bytes are read and 1 written per element; the quotients
+// take about as long as the bytes do (SM throughput 77% at 76% of the copy rate).
 //
 // Measured: 8 prompts of 4096 rows, 8 heads of dim 128 (205 MB) 41.5 us, 4.9
 // TB/s (60 us where blocks of new rows had row checks as well, 75 us with 512

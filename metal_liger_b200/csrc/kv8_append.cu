@@ -4,10 +4,10 @@
 // With a = max |x| over the block's live values x,
 //   scale = a / qmax,   code = round(x * qmax / a)      (qmax: 127, or 448 for e4m3)
 // rounded half to even to an integer, or to the nearest e4m3 value.  x has at
-// most 11 significant bits and qmax 7, so x * qmax is exact in fp32, the one
-// IEEE division is correctly rounded, and it is a tie exactly where
-// the true quotient is one (two such ratios that differ do so by more than
-// 2^-22 of their size): every code is the one the formula gives in exact
+// most 11 significant bits and qmax 7, so x * qmax is exact in fp32, the
+// quotient is correctly rounded, and so it is a tie exactly where the true one
+// is (two such ratios that differ do so by more than 2^-22 of their size): every
+// code is the one the formula gives in exact
 // arithmetic.  A block without a non-zero value has scale 0 and codes 0; a
 // block holding an infinity or NaN gets that as its scale and codes 0, so it
 // reads back as NaN.

@@ -20,10 +20,17 @@
 //
 // Queries enter as fp16 scaled by a power of two per row (bf16 and fp16 fit
 // exactly down to 2^-14 of the row's largest value, and to 2^-25 of it below).
-// Probabilities are fp16 in [0, 1], sums and outputs fp32.  The scale of a V
-// block enters the exponent: the output keeps its own running reference
-// Mo = max(s + log2 vscale), so weights 2^(s + log2 vscale - Mo) stay in
-// [0, 1] however far the block scales lie apart.
+// Sums, statistics and outputs are fp32.  The scale of a V block enters the
+// exponent: the output keeps its own running reference Mo = max(s + log2
+// vscale), so weights 2^(s + log2 vscale - Mo) stay in [0, 1] however far the
+// block scales lie apart.  For the second product they are rounded to fp16
+// (what mma.sync takes beside the codes), times 2^15, which the output is
+// divided by: the largest is 2^15 and fp16's normal range ends at 2^-29 of it,
+// its smallest step at 2^-39, so a long tail behind one dominant position
+// keeps its weight (the denominator counts it in fp32).  With the largest at 1,
+// outputs that are the tail behind a position with 0.9999 of the weight were 1.1%
+// off (8192 positions, dim 256); the factor is one addition per tile, and its
+// time does not show (64 sequences of up to 8192: 102.6 us, 103.2 before).
 //
 // Work is divided evenly whatever the lengths: all 32-position tiles of all
 // (sequence, kv head, row tile) segments form one flat list, each CTA takes an
@@ -41,6 +48,8 @@ namespace ml {
 namespace {
 
 constexpr int kTile = 32;  // positions per warp step
+constexpr float kUpLog2 = 15.f;       // of the weights in fp16 ...
+constexpr float kDown = 0x1p-15f;     // ... and back
 
 struct AttnArgs {
   const void* q;            // [B, Hq, T, D] at element strides
@@ -287,8 +296,8 @@ struct State {
           uint32_t w[PER / 2];
 #pragma unroll
           for (int j = 0; j < PER / 2; ++j) {
-            const float lo = none ? 0.f : acc[n][p * 8 + j][c] * f;
-            const float hi = none ? 0.f : acc[n][p * 8 + j][2 + c] * f;
+            const float lo = none ? 0.f : acc[n][p * 8 + j][c] * kDown * f;
+            const float hi = none ? 0.f : acc[n][p * 8 + j][2 + c] * kDown * f;
             T two[2] = {from_f32<T>(lo), from_f32<T>(hi)};
             memcpy(&w[j], two, 4);
           }
@@ -464,7 +473,7 @@ __device__ __forceinline__ void score_step(State<D, NT>& st, const Query<D, NT>&
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const float m = st.m[n][c] == -INFINITY ? 0.f : st.m[n][c];
-      const float o = lv - (st.mo[n][c] == -INFINITY ? 0.f : st.mo[n][c]);
+      const float o = lv + kUpLog2 - (st.mo[n][c] == -INFINITY ? 0.f : st.mo[n][c]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -626,7 +635,7 @@ __device__ __forceinline__ void write_item(const AttnArgs& a, int b, int seg, in
     T* dst = static_cast<T*>(a.out) +
              (((int64_t)b * a.span.tokens + tok) * (a.kv_heads * a.group) + h) * D +
              (j * 2 / PER) * 128 + g * PER + j * 2 % PER;
-    T two[2] = {from_f32<T>(o[c]), from_f32<T>(o[2 + c])};
+    T two[2] = {from_f32<T>(o[c] * kDown), from_f32<T>(o[2 + c] * kDown)};
     uint32_t w;
     memcpy(&w, two, 4);
     *reinterpret_cast<uint32_t*>(dst) = w;

@@ -667,8 +667,10 @@ ML_API int ml_gemv_rmsnorm_swiglu_bf16(const void* x, int64_t ld_x, const void* 
  * ([batch, kv_heads, max_len / block]); value = code * scale.  k_tail / v_tail
  * [batch, kv_heads, 2, block, head_dim] in `dtype` (ML_DTYPE_BF16 or
  * ML_DTYPE_F16, the type of k, v, q and the output) keep the unquantised rows
- * of the last two blocks written, block i in slot i & 1.  All contiguous;
- * codes and tails 16-byte aligned; head_dim 64, 128 or 256; block 32, 64 or
+ * of the last two blocks of each append, block i in slot i & 1; k_held / v_held
+ * [batch, kv_heads, 2] which block that is in each slot (negative: not known,
+ * as before the first append), or NULL.  All contiguous; codes and tails 16-byte,
+ * k_held and v_held 8-byte aligned; head_dim 64, 128 or 256; block 32, 64 or
  * 128; max_len a multiple of block.
  */
 #define ML_KV8_INT8 0
@@ -683,6 +685,8 @@ typedef struct ml_kv8_cache {
   int format;
   int dtype;
   int64_t batch, kv_heads, max_len, head_dim, block;
+  int32_t* k_held; /* only the append uses them; both or neither */
+  int32_t* v_held;
 } ml_kv8_cache;
 
 /*
@@ -695,9 +699,14 @@ typedef struct ml_kv8_cache {
  * scale = a / qmax (qmax 127, e4m3 448), code = round(x * qmax / a), half to
  * even; a block holding inf or NaN reads back as NaN.  Rows that would pass
  * max_len, and sequences whose start is negative or past max_len, write
- * nothing.  A start inside a block needs that block's earlier rows to be in
- * the tail: they are after any append that ended in this block or the next.
- * Positions past the last new row keep what they held.
+ * nothing.  A start inside a block takes that block's earlier rows from the
+ * tail.  Its slot has them if, of all appends that wrote to a block of the same
+ * parity as one of their last two, the latest had this block among them; so
+ * steps forward always find them, and steps back to a border need none.  Where
+ * the slot has another block, the earlier rows are their codes' values rounded to
+ * `dtype` if k_held / v_held are there to show it; without them the append takes
+ * the slot's rows for the block's own.  The codes of positions past the last new
+ * row stay as they were (under the scale that their block then has).
  */
 ML_API int ml_kv8_append(const ml_kv8_cache* cache, const void* k, const int64_t* k_strides,
                          const void* v, const int64_t* v_strides, int64_t tokens,

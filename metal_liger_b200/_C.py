@@ -69,7 +69,8 @@ class Kv8Cache(ctypes.Structure):
     _fields_ = [("k_codes", c_void_p), ("v_codes", c_void_p), ("k_scale", c_void_p),
                 ("v_scale", c_void_p), ("k_tail", c_void_p), ("v_tail", c_void_p),
                 ("format", c_int), ("dtype", c_int), ("batch", c_int64), ("kv_heads", c_int64),
-                ("max_len", c_int64), ("head_dim", c_int64), ("block", c_int64)]
+                ("max_len", c_int64), ("head_dim", c_int64), ("block", c_int64),
+                ("k_held", c_void_p), ("v_held", c_void_p)]
 
 
 # name -> (restype, argtypes).  Kept in the same order as the header.

@@ -1049,19 +1049,27 @@ def _kv8_index(name: str, what: str, t: Tensor | None, batch: int):
 
 def kv8_append_cuda(k: Tensor, v: Tensor, start: Tensor, counts: Tensor | None, k_codes: Tensor,
                     v_codes: Tensor, k_scale: Tensor, v_scale: Tensor, k_tail: Tensor,
-                    v_tail: Tensor) -> None:
+                    v_tail: Tensor, held: Tensor | None = None) -> None:
     """Append k, v [B, Hkv, T, D] (bf16 or fp16) at positions ``start`` + t of
     each sequence (rows t >= ``counts`` are padding) to a cache held in 8
-    bits, in place."""
+    bits, in place.  ``held`` (int32 [2, B, Hkv, 2], of K and of V): which block
+    each tail slot has."""
     name = "kv8_append"
     dev = _same_device(name, k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail,
-                       v_tail)
+                       v_tail, held)
     c = _kv8_cache(name, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail, k.dtype)
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or shape[0] != c.batch or \
             shape[1] != c.kv_heads or shape[3] != c.head_dim:
         raise RuntimeError(f"{name}: k {tuple(k.shape)} and v {tuple(v.shape)} do not match the "
                            f"cache {tuple(k_codes.shape)}")
+    if held is not None:
+        if held.dtype != torch.int32 or held.shape != (2, c.batch, c.kv_heads, 2) or \
+                not held.is_contiguous():
+            raise RuntimeError(f"{name}: held must be int32 (2, {c.batch}, {c.kv_heads}, 2), not "
+                               f"{held.dtype} {tuple(held.shape)}")
+        c.k_held = held.data_ptr()
+        c.v_held = c.k_held + 8 * c.batch * c.kv_heads
     sp, ss = _kv8_index(name, "start", start, shape[0])
     cp, cs = _kv8_index(name, "counts", counts, shape[0])
     with _C.on_device(dev):
@@ -1138,7 +1146,8 @@ def sample_cuda(logits: Tensor, uniform: Tensor, temperature: Tensor | None,
 _SCHEMAS = {
     "kv8_append": "kv8_append(Tensor k, Tensor v, Tensor start, Tensor? counts, "
                   "Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) k_scale, "
-                  "Tensor(d!) v_scale, Tensor(e!) k_tail, Tensor(f!) v_tail) -> ()",
+                  "Tensor(d!) v_scale, Tensor(e!) k_tail, Tensor(f!) v_tail, "
+                  "Tensor(g!)? held=None) -> ()",
     "kv8_attention": "kv8_attention(Tensor q, Tensor start, Tensor? counts, Tensor k_codes, "
                      "Tensor v_codes, Tensor k_scale, Tensor v_scale, Tensor k_tail, "
                      "Tensor v_tail, float scale) -> Tensor",
@@ -1361,7 +1370,8 @@ def _fake_impls():
         B, Hkv, L, D = k_cache.shape
         return torch.empty((B, q.numel() // (B * D), 1, D), dtype=q.dtype, device=q.device)
 
-    def kv8_append_fake(k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail):
+    def kv8_append_fake(k, v, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail,
+                        held=None):
         return None
 
     def kv8_attention_fake(q, start, counts, k_codes, v_codes, k_scale, v_scale, k_tail, v_tail,

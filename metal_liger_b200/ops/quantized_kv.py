@@ -4,7 +4,8 @@ No counterpart in the reference, whose static cache keeps the model's dtype
 (generation.py:18-66).  One layer's cache is a ``QuantizedKV`` of six device
 buffers: int8 or e4m3 codes for K and V, one fp32 scale for each block of
 positions and kv head, and the unquantised rows of the last two blocks (the
-"tail"), so that a block is always quantised from its values themselves:
+"tail"), so that a block that is written on is quantised from its values
+themselves:
 
     a = max |x| over the block,   scale = a / qmax,   code = round(x * qmax / a)
 
@@ -32,15 +33,24 @@ CACHE_DTYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 DEFAULT_BLOCK = 64
 
 
-class QuantizedKV(NamedTuple):
-    """One layer's cache buffers."""
-
+class _Buffers(NamedTuple):
     k_codes: Tensor   # [B, Hkv, L, D] int8 or float8_e4m3fn
     k_scale: Tensor   # [B, Hkv, L / block] float32
     k_tail: Tensor    # [B, Hkv, 2, block, D] bf16 or fp16
     v_codes: Tensor
     v_scale: Tensor
     v_tail: Tensor
+
+
+class QuantizedKV(_Buffers):
+    """One layer's cache buffers.
+
+    ``held`` (int32 [2, B, Hkv, 2]; K, V): which block each slot of the tails
+    has, negative where that is not known.  ``allocate_quantized_kv`` makes it; a
+    cache put together from buffers (``_replace`` among them) has none, and its
+    appends take the tails for the rows of whatever block they continue."""
+
+    held: Optional[Tensor] = None
 
     @property
     def max_len(self) -> int:
@@ -83,7 +93,9 @@ def allocate_quantized_kv(batch: int, kv_heads: int, max_len: int, head_dim: int
                 torch.zeros((*shape, length // block), dtype=torch.float32, device=device),
                 torch.zeros((*shape, 2, block, head_dim), dtype=dtype, device=device))
 
-    return QuantizedKV(*half(), *half())
+    kv = QuantizedKV(*half(), *half())
+    kv.held = torch.full((2, *shape, 2), -1, dtype=torch.int32, device=device)
+    return kv
 
 
 def _eager(t: Tensor) -> bool:
@@ -97,15 +109,23 @@ def quantized_kv_append(kv: QuantizedKV, k: Tensor, v: Tensor, start: Tensor,
     ``counts`` (int64): how many of the T rows are real in each sequence, the
     others being padding.  Blocks that get a row are requantised whole; rows
     past ``max_len`` are dropped, as are those of a sequence whose start is
-    negative; positions past the last new one keep what they held.
+    negative; the codes of positions past the last new one stay as they were.
 
-    ``start`` may go back (a drafted continuation rejected, a new prompt at 0):
-    to any block border, or into a block that is the last one written or the
-    one before it, whose unquantised rows the tail still has."""
+    ``start`` may go back (a drafted continuation rejected, a new prompt at 0).
+    From a block border, and inside a block whose unquantised rows the tail
+    still has, the cache is that of one call with all the rows.  The tail has
+    the last two blocks of each append, odd and even ones in a slot of their own:
+    a sequence that only goes forward, or goes back once into the block it ended
+    in or the one before, always finds its rows there.  After a further step
+    back the slot may have a later block: then the older rows are what their
+    codes stand for, rounded to the rows' dtype, which leaves their codes as they
+    are while the block's largest value stands.  (A cache without ``kv.held``
+    cannot tell, and needs ``start`` to be one of the others.)"""
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise RuntimeError("quantized_kv_append has no backward: call it under torch.no_grad()")
     op = _tl.kv8_append_cuda if _eager(k) else torch.ops.metal_liger.kv8_append
-    op(k, v, start, counts, kv.k_codes, kv.v_codes, kv.k_scale, kv.v_scale, kv.k_tail, kv.v_tail)
+    op(k, v, start, counts, kv.k_codes, kv.v_codes, kv.k_scale, kv.v_scale, kv.k_tail, kv.v_tail,
+       kv.held)
 
 
 def quantized_kv_attention(q: Tensor, kv: QuantizedKV, start: Tensor,

@@ -43,7 +43,10 @@ forward returns ``last_hidden_state``) and a bias-free or biased
 from __future__ import annotations
 
 import contextlib
+import functools
 import logging
+import sys
+import threading
 from collections import OrderedDict
 from typing import Optional
 
@@ -248,8 +251,29 @@ class _QuantizedKVLayer(_StaticKVLayer):
         self.max_cache_len = owner.max_seq_len
 
 
-_KV8_ATTN = "metal_liger_kv8"
-_KV8_CACHE: list = [None]
+class _ThreadSlot(threading.local):
+    """One value for each thread, as slot[0]: several threads may generate, each
+    with a model of its own."""
+
+    value = None
+
+    def __getitem__(self, _):
+        return self.value
+
+    def __setitem__(self, _, value):
+        self.value = value
+
+
+# The quantised cache whose step this thread decodes.
+_KV8_CACHE = _ThreadSlot()
+
+
+def _kv8_answers(module) -> bool:
+    """Whether this call of `module`'s attention follows an update() of the
+    thread's quantised cache."""
+    cache = _KV8_CACHE[0]
+    return (cache is not None and cache.pending is not None
+            and getattr(module, "layer_idx", None) in cache.pending)
 
 
 def _windowed(window: Optional[int], cache) -> bool:
@@ -261,11 +285,10 @@ def _kv8_attention_forward(module, query, key, value, attention_mask, dropout=0.
                            **kwargs):
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
 
-    cache = _KV8_CACHE[0]
-    layer = getattr(module, "layer_idx", None)
-    if cache is None or cache.pending is None or layer not in cache.pending:
+    if not _kv8_answers(module):
         return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
                                       scaling=scaling, **kwargs)
+    cache, layer = _KV8_CACHE[0], module.layer_idx
     cache.pending.discard(layer)
     extra = [n for n in ("softcap", "s_aux") if kwargs.get(n) is not None]
     if _windowed(kwargs.get("sliding_window"), cache):
@@ -290,12 +313,11 @@ class _QuantizedAttention:
     def __enter__(self):
         if self.cache is None:
             return self
-        self.attn_prev = getattr(self.config, "_attn_implementation", None)
-        self.cache_prev = _KV8_CACHE[0]
-        if self.attn_prev is None:
+        if getattr(self.config, "_attn_implementation", None) is None:
             raise RuntimeError("kv_cache_dtype: the decoder has no attention implementation to "
                                "replace (config._attn_implementation)")
-        self.config._attn_implementation = _KV8_ATTN
+        _swap_attention(self.config)
+        self.cache_prev = _KV8_CACHE[0]
         _KV8_CACHE[0] = self.cache
         self.cache.pending = set()
         return self
@@ -304,8 +326,8 @@ class _QuantizedAttention:
         if self.cache is None:
             return False
         left, self.cache.pending = self.cache.pending, None
-        self.config._attn_implementation = self.attn_prev
         _KV8_CACHE[0] = self.cache_prev
+        _restore_attention(self.config)
         if left and exc_type is None:
             raise RuntimeError(f"kv_cache_dtype: layers {sorted(left)} did not attend through "
                                "transformers' attention interface")
@@ -314,18 +336,23 @@ class _QuantizedAttention:
 
 # Decode-step attention: registered with transformers' attention interface
 # under this name and selected on the decoder's config while the decode step
-# is captured.  It reads the number of filled positions from the device-side
-# position the captured step advances (_DECODE_POS), so the attention needs
-# neither a mask nor repeat_kv copies; any other call (prefill, several
-# query tokens, other dtypes) goes to transformers' SDPA path unchanged.
+# is captured, or run over a quantised cache.  Over the plain cache it reads the
+# number of filled positions from the device-side position the captured step
+# advances (_DECODE_POS), so the attention needs neither a mask nor repeat_kv
+# copies; any other call (prefill, several query tokens, other dtypes, another
+# thread's) goes to transformers' SDPA path unchanged, under the mask that this
+# path is given.
 _DECODE_ATTN = "metal_liger_decode"
-_DECODE_POS: list = [None]
+_DECODE_POS = _ThreadSlot()
 
 
 def _decode_attention_forward(module, query, key, value, attention_mask, dropout=0.0,
                               scaling=None, **kwargs):
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
 
+    if _kv8_answers(module):
+        return _kv8_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
+                                      scaling=scaling, **kwargs)
     pos = _DECODE_POS[0]
     D = query.shape[-1]
     G = query.shape[1] // key.shape[1] if key.dim() == 4 and key.shape[1] else 0
@@ -340,13 +367,73 @@ def _decode_attention_forward(module, query, key, value, attention_mask, dropout
     return out, None
 
 
+def _other_attention_forward(implementation, module, *args, **kwargs):
+    """The step's attention in the place of an implementation other than SDPA."""
+    if _kv8_answers(module):
+        return _kv8_attention_forward(module, *args, **kwargs)
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+    if implementation in ALL_ATTENTION_FUNCTIONS:
+        forward = ALL_ATTENTION_FUNCTIONS[implementation]
+    else:  # "eager": each modeling module has its own
+        forward = sys.modules[type(module).__module__].eager_attention_forward
+    return forward(module, *args, **kwargs)
+
+
+# Configs whose attention implementation is replaced: [config, what it was, by how
+# many].  Threads may share a model, and any of them may be the last to leave.
+_SWAPS: dict = {}
+_SWAP_LOCK = threading.Lock()
+
+
+def _attention_of(config) -> Optional[str]:
+    """The config's own attention implementation, replaced or not."""
+    entry = _SWAPS.get(id(config))
+    return entry[1] if entry is not None else getattr(config, "_attn_implementation", None)
+
+
+def _swap_attention(config) -> None:
+    with _SWAP_LOCK:
+        entry = _SWAPS.get(id(config))
+        if entry is None:
+            prev = config._attn_implementation
+            config._attn_implementation = _decode_name(prev)
+            entry = _SWAPS[id(config)] = [config, prev, 0]
+        entry[2] += 1
+
+
+def _restore_attention(config) -> None:
+    with _SWAP_LOCK:
+        entry = _SWAPS[id(config)]
+        entry[2] -= 1
+        if entry[2] == 0:
+            config._attn_implementation = entry[1]
+            del _SWAPS[id(config)]
+
+
+def _decode_name(implementation: str) -> str:
+    """The registered name of the step's attention in the place of another: calls
+    that are not the step's keep that one, and are given the masks it is given."""
+    if implementation == "sdpa":
+        return _DECODE_ATTN
+    from transformers import AttentionInterface, AttentionMaskInterface
+    from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
+
+    name = f"{_DECODE_ATTN}_{implementation}"
+    if implementation in ALL_MASK_ATTENTION_FUNCTIONS:
+        AttentionMaskInterface.register(name, ALL_MASK_ATTENTION_FUNCTIONS[implementation])
+    AttentionInterface.register(name, functools.partial(_other_attention_forward, implementation))
+    return name
+
+
 def _register_decode_attention() -> bool:
     try:
-        from transformers import AttentionInterface
+        from transformers import AttentionInterface, AttentionMaskInterface
+        from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
     except ImportError:  # pragma: no cover - transformers is part of the image
         return False
     AttentionInterface.register(_DECODE_ATTN, _decode_attention_forward)
-    AttentionInterface.register(_KV8_ATTN, _kv8_attention_forward)
+    AttentionMaskInterface.register(_DECODE_ATTN, ALL_MASK_ATTENTION_FUNCTIONS["sdpa"])
     return True
 
 
@@ -372,7 +459,7 @@ class _DecodeKernels:
         self.gemv = gemv
         self.cache = cache
         self.patched = []
-        self.attn_prev = None
+        self.swapped = None
 
     def __enter__(self):
         from metal_liger_b200 import _torch_library  # noqa: F401  (registers the ops)
@@ -380,9 +467,9 @@ class _DecodeKernels:
         cfg = getattr(self.module, "config", None)
         quantized = isinstance(self.cache, MetalLigerQuantizedCache)
         if self.pos is not None and cfg is not None and not quantized and \
-                getattr(cfg, "_attn_implementation", None) == "sdpa":
-            self.attn_prev = cfg._attn_implementation
-            cfg._attn_implementation = _DECODE_ATTN
+                _attention_of(cfg) == "sdpa":
+            _swap_attention(cfg)
+            self.swapped = cfg
             _DECODE_POS[0] = self.pos
 
         from metal_liger_b200.ops.fused_swiglu import MetalLigerSwiGLU
@@ -435,9 +522,9 @@ class _DecodeKernels:
         for mod in self.patched:
             del mod.forward
         self.patched = []
-        if self.attn_prev is not None:
-            self.module.config._attn_implementation = self.attn_prev
-            self.attn_prev = None
+        if self.swapped is not None:
+            _restore_attention(self.swapped)
+            self.swapped = None
         _DECODE_POS[0] = None
         return False
 
@@ -447,8 +534,6 @@ def _decode_block_ok(attn, cache) -> bool:
     plain bf16 linears, q_norm / k_norm this library's RMSNorm, RoPE rebound
     to this library's kernel (so the arithmetic is the model's own eager
     path's), and head shapes the decode kernels take."""
-    import sys
-
     from metal_liger_b200.ops.fused_rms_norm import MetalLigerRMSNorm
     from metal_liger_b200.patch import _fused_rotary_pos_emb
 
@@ -756,8 +841,9 @@ class MetalLigerGenerator:
         # decoder would otherwise read at capture time
         extra = {"position_ids": (pos.view(1, 1, 1).expand(3, B, 1) if self._mrope
                                   else pos.view(1, 1).expand(B, 1))}
-        h = self.decoder(input_ids=tok, attention_mask=mask, past_key_values=cache,
-                         use_cache=True, return_dict=True, **extra).last_hidden_state[:, -1, :]
+        with _QuantizedAttention(self.decoder, cache):
+            h = self.decoder(input_ids=tok, attention_mask=mask, past_key_values=cache,
+                             use_cache=True, return_dict=True, **extra).last_hidden_state[:, -1, :]
         if st["sampling"] is None:
             tok.copy_(self._greedy(h).view(B, 1))
         else:
@@ -807,11 +893,9 @@ class MetalLigerGenerator:
         HBM-streaming GEMV while the step is built (batch <= 2)."""
         B = st.ids.shape[0]
         if capture and st.graph is None:
-            with _DecodeKernels(self.decoder, st.pos, gemv=B <= 2, cache=st.cache), \
-                    _QuantizedAttention(self.decoder, st.cache):
+            with _DecodeKernels(self.decoder, st.pos, gemv=B <= 2, cache=st.cache):
                 return self._decode_static_inner(st, n, steps, eos_token_id, capture)
-        with _QuantizedAttention(self.decoder, st.cache):
-            return self._decode_static_inner(st, n, steps, eos_token_id, capture)
+        return self._decode_static_inner(st, n, steps, eos_token_id, capture)
 
     def _decode_static_inner(self, st: "_DecodeState", n, steps, eos_token_id,
                              capture: bool) -> int:
@@ -881,6 +965,11 @@ class MetalLigerGenerator:
         the step; the tokens are the same as the eager loop's up to
         near-ties at the logits' rounding (the attention then runs over the
         full static buffers under a mask).
+
+        Threads may generate at the same time, each with a model and a generator
+        of its own, once their steps are captured (or with ``cuda_graph=False``):
+        CUDA lets no other thread allocate or draw random numbers during a
+        capture, which a generator makes in its first call of a size.
 
         The keyword-only arguments are not in the reference either.
         ``kv_cache_dtype`` "int8" or "fp8" holds the KV cache in 8 bits; decode

@@ -13,6 +13,7 @@ import torch
 from torch import Tensor
 
 from metal_liger_b200 import _torch_library as _tl
+from metal_liger_b200.ops.quantized_kv import refuse_derivatives
 
 
 def _split(name: str, x, ok):
@@ -47,8 +48,7 @@ def fused_sample(logits: Tensor, uniform: Tensor, temperature: Union[float, Tens
     k, kv = _split("top_k", top_k, lambda x: x >= 0)
     p, pv = _split("top_p", top_p, lambda x: 0.0 <= x <= 1.0)
     m, mv = _split("min_p", min_p, lambda x: 0.0 <= x <= 1.0)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        raise RuntimeError("fused_sample has no backward: call it under torch.no_grad()")
+    refuse_derivatives("fused_sample", logits, uniform, t, k, p, m)
     eager = logits.is_cuda and type(logits) is Tensor and not torch.compiler.is_compiling()
     op = _tl.sample_cuda if eager else torch.ops.metal_liger.sample
     return op(logits, uniform, t, tv, k, kv, p, pv, m, mv)

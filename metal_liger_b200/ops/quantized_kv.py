@@ -26,6 +26,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from metal_liger_b200 import _torch_library as _tl
 
@@ -98,6 +99,22 @@ def allocate_quantized_kv(batch: int, kv_heads: int, max_len: int, head_dim: int
     return kv
 
 
+def refuse_derivatives(name: str, *tensors: Optional[Tensor]) -> None:
+    """Raises where a derivative through ``tensors`` is asked for, in reverse mode
+    (one requires grad) or forward mode (one is a dual tensor): it would be
+    dropped without a word."""
+    # (outside any forward-mode level, -1, there are no dual tensors to look for)
+    forward = getattr(forward_ad, "_current_level", 0) >= 0
+    reverse = torch.is_grad_enabled()
+    for t in tensors:
+        if t is None:
+            continue
+        if reverse and t.requires_grad:
+            raise RuntimeError(f"{name} has no backward: call it under torch.no_grad()")
+        if forward and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative: call it on the primals")
+
+
 def _eager(t: Tensor) -> bool:
     return t.is_cuda and type(t) is Tensor and not torch.compiler.is_compiling()
 
@@ -121,8 +138,7 @@ def quantized_kv_append(kv: QuantizedKV, k: Tensor, v: Tensor, start: Tensor,
     codes stand for, rounded to the rows' dtype, which leaves their codes as they
     are while the block's largest value stands.  (A cache without ``kv.held``
     cannot tell, and needs ``start`` to be one of the others.)"""
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
-        raise RuntimeError("quantized_kv_append has no backward: call it under torch.no_grad()")
+    refuse_derivatives("quantized_kv_append", k, v)
     op = _tl.kv8_append_cuda if _eager(k) else torch.ops.metal_liger.kv8_append
     op(k, v, start, counts, kv.k_codes, kv.v_codes, kv.k_scale, kv.v_scale, kv.k_tail, kv.v_tail,
        kv.held)
@@ -137,9 +153,7 @@ def quantized_kv_attention(q: Tensor, kv: QuantizedKV, start: Tensor,
     the append of the same tokens; Hq is a multiple of the cache's kv heads.
     Rows t >= ``counts`` and rows that see nothing are zeros.  ``scale``
     defaults to D ** -0.5."""
-    if torch.is_grad_enabled() and q.requires_grad:
-        raise RuntimeError("quantized_kv_attention has no backward: call it under "
-                           "torch.no_grad()")
+    refuse_derivatives("quantized_kv_attention", q)
     op = _tl.kv8_attention_cuda if _eager(q) else torch.ops.metal_liger.kv8_attention
     return op(q, start, counts, kv.k_codes, kv.v_codes, kv.k_scale, kv.v_scale, kv.k_tail,
               kv.v_tail, q.shape[-1] ** -0.5 if scale is None else scale)

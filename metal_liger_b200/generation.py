@@ -26,8 +26,8 @@ On B200:
   which skips its per-forward device-to-host sync;
 * the sampling step takes its logits from this library's GEMM (bf16, the
   logit dtype of a bf16 model) and samples with torch, or, with
-  ``fused_sampling`` (or ``top_k`` / ``min_p``, which the reference lacks),
-  with this library's sampler, which honours ``top_p`` and runs inside the
+  ``fused_sampling`` (or a ``top_k`` / ``min_p`` that filters; the reference
+  has neither), with this library's sampler, which honours ``top_p`` and runs inside the
   captured decode step;
 * with ``kv_cache_dtype`` "int8" or "fp8" the cache is held in 8 bits
   (``MetalLigerQuantizedCache``): half the memory per position, and half the
@@ -975,11 +975,12 @@ class MetalLigerGenerator:
         ``kv_cache_dtype`` "int8" or "fp8" holds the KV cache in 8 bits; decode
         steps then attend to every position before them, so a mask that hides
         some (padding) and sliding windows are refused.
-        ``fused_sampling`` (implied by ``top_k`` or ``min_p``) draws every token,
-        the first included, with ``ops.fused_sampling`` from ``temperature``,
-        ``top_k``, ``top_p`` and ``min_p``, all honoured (temperature 0 is
-        greedy), on the captured step as well; ``generator`` (a CUDA
-        ``torch.Generator``) gives its uniform numbers."""
+        ``fused_sampling`` (implied by a ``top_k`` or ``min_p`` other than 0, which
+        filters nothing) draws every token, the first included, with
+        ``ops.fused_sampling`` from ``temperature``, ``top_k``, ``top_p`` and
+        ``min_p``, all honoured (temperature 0 is greedy), on the captured step as
+        well; ``generator`` (a CUDA ``torch.Generator``) gives its uniform
+        numbers."""
         batch_size, prompt_len = input_ids.shape
         max_len = prompt_len + max_new_tokens
         if kv_cache_dtype is not None:
@@ -987,7 +988,8 @@ class MetalLigerGenerator:
             if seen is not None and (seen.dim() != 2 or not bool((seen != 0).all())):
                 raise ValueError("generate: kv_cache_dtype takes no padded batch and no attention "
                                  "mask of its own")
-        fused = (fused_sampling or top_k is not None or min_p is not None) and temperature != 0
+        _check_sampling(1.0, int(top_k or 0), 1.0, float(min_p or 0.0))
+        fused = (fused_sampling or bool(top_k) or bool(min_p)) and temperature != 0
         greedy = not fused and (temperature == 0 or (temperature == 1.0 and top_p == 1.0))
         if cuda_graph is None:
             cuda_graph = (input_ids.device.type == "cuda"

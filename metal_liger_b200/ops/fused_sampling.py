@@ -45,7 +45,7 @@ def fused_sample(logits: Tensor, uniform: Tensor, temperature: Union[float, Tens
     -inf are never taken, and a row of nothing else gives id -1, logprob
     -inf."""
     t, tv = _split("temperature", temperature, lambda x: 0.0 <= x < math.inf)
-    k, kv = _split("top_k", top_k, lambda x: x >= 0)
+    k, kv = _split("top_k", top_k, lambda x: 0 <= x < 2 ** 63)  # an int64
     p, pv = _split("top_p", top_p, lambda x: 0.0 <= x <= 1.0)
     m, mv = _split("min_p", min_p, lambda x: 0.0 <= x <= 1.0)
     refuse_derivatives("fused_sample", logits, uniform, t, k, p, m)

@@ -1040,7 +1040,9 @@ int launch_kernel(const AttnArgs& a, int64_t grid, cudaStream_t st) {
 template <typename T, int FMT, int D, int NT>
 int launch(AttnArgs a, cudaStream_t st) {
   const int64_t segs = (int64_t)a.batch * a.kv_heads * a.row_tiles;
-  ML_CHECK_ARG(segs * (a.max_len / kTile + kPad) < ((int64_t)1 << 31),
+  // (below 2^31 by more than what a warp's `first tile + share` can pass the total
+  // by: the CTAs' shares are rounded up to whole tiles, and so are the warps')
+  ML_CHECK_ARG(segs * (a.max_len / kTile + kPad) < ((int64_t)1 << 31) - ((int64_t)1 << 17),
                "kv8_attention: too many query rows for this cache in one call");
   if constexpr (NT == 1) {
     if (a.part == nullptr) return launch_kernel<T, FMT, D, 1, segment_warps(D)>(a, segs, st);

@@ -8,9 +8,12 @@
 // head against 4 D flops per query head.  So a warp converts 32 positions of
 // K and V to fp16 in registers (exact: codes have at most 8 bits) and lets
 // mma.sync do both products for up to 8 NT query rows of the kv head at a
-// time; with at most 16 rows to a tile a tcgen05 tile of 64 or 128 rows would
-// be mostly padding, and its operands would have to go back through shared
-// memory after the conversion.
+// time: it takes the operands from the registers that the conversion leaves them
+// in, where tcgen05 (positions as M, query rows as N) would have them written to
+// shared memory or TMEM first.  For one token that is no bound (long caches run at
+// 87% of the copy rate).  Many query tokens convert the codes again for every 8 or
+// 16 rows and get a tenth of the tensor rate: 4 sequences, 256 tokens of 32 heads
+// over 4000 positions take 391 us, 172 TFLOP/s.
 //   S^T = K Q^T:  A = 16 positions x 16 dims, B = 16 dims x 8 query rows
 //   O^T = V^T P^T: A = 16 dims x 16 positions, B = 16 positions x 8 query rows
 // Any order of the summed index serves as long as both operands agree on it,
@@ -1001,6 +1004,10 @@ inline int n_tiles(const ml_kv8_cache* c, int64_t rows) {
 // (one such CTA fills an SM).  One launch against the list, 64 segments: 250
 // positions 7.3 us / 13.1, 1000 11.6 / 13.7, 2000 16.1 / 16.1; 8 segments: 1000
 // 11.4 / 10.9, 2000 15.7 / 11.4; 256 segments: 250 14.5 / 14.5, 500 17.8 / 16.6.
+// The rule goes by the capacity, since only the device knows how far a cache is
+// filled: of 4096 positions, 250 of them filled, 64 segments take the list, 13.2
+// us, where a cache of 256 takes one launch, 7.2 (8 segments 10.7, 6.8); 1000
+// filled, 13.7 and 11.7 (10.9, 11.3).
 constexpr int64_t kOneLaunchLen = 1024;
 
 struct Plan {

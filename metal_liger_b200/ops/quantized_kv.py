@@ -51,7 +51,16 @@ class QuantizedKV(_Buffers):
     cache put together from buffers (``_replace`` among them) has none, and its
     appends take the tails for the rows of whatever block they continue."""
 
-    held: Optional[Tensor] = None
+    held: Optional[Tensor]
+
+    def __new__(cls, *args, **kwargs):
+        self = super().__new__(cls, *args, **kwargs)
+        self.held = None  # (an attribute of each instance, as torch.compile guards it)
+        return self
+
+    @classmethod
+    def _make(cls, iterable):
+        return cls(*iterable)
 
     @property
     def max_len(self) -> int:

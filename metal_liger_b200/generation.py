@@ -380,6 +380,15 @@ def _other_attention_forward(implementation, module, *args, **kwargs):
     return forward(module, *args, **kwargs)
 
 
+def _other_mask(mask, *args, **kwargs):
+    """The masks of calls that are not the step's; the step over a quantised cache
+    looks at none, and none is made for it."""
+    cache = _KV8_CACHE[0]
+    if cache is not None and cache.pending is not None:
+        return None
+    return mask(*args, **kwargs)
+
+
 # Configs whose attention implementation is replaced: [config, what it was, by how
 # many].  Threads may share a model, and any of them may be the last to leave.
 _SWAPS: dict = {}
@@ -421,7 +430,8 @@ def _decode_name(implementation: str) -> str:
 
     name = f"{_DECODE_ATTN}_{implementation}"
     if implementation in ALL_MASK_ATTENTION_FUNCTIONS:
-        AttentionMaskInterface.register(name, ALL_MASK_ATTENTION_FUNCTIONS[implementation])
+        AttentionMaskInterface.register(name, functools.partial(
+            _other_mask, ALL_MASK_ATTENTION_FUNCTIONS[implementation]))
     AttentionInterface.register(name, functools.partial(_other_attention_forward, implementation))
     return name
 
@@ -433,7 +443,8 @@ def _register_decode_attention() -> bool:
     except ImportError:  # pragma: no cover - transformers is part of the image
         return False
     AttentionInterface.register(_DECODE_ATTN, _decode_attention_forward)
-    AttentionMaskInterface.register(_DECODE_ATTN, ALL_MASK_ATTENTION_FUNCTIONS["sdpa"])
+    AttentionMaskInterface.register(_DECODE_ATTN, functools.partial(
+        _other_mask, ALL_MASK_ATTENTION_FUNCTIONS["sdpa"]))
     return True
 
 

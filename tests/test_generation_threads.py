@@ -201,3 +201,19 @@ def test_replays_leave_the_config_alone():
 
     assert g._decode_static(State, 3, 4, None, capture=True) == 7
     assert seen == [("sdpa", None)] * 4
+
+
+def test_no_mask_is_made_for_the_step(monkeypatch):
+    from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
+
+    made = ALL_MASK_ATTENTION_FUNCTIONS[G._DECODE_ATTN]
+    kw = dict(batch_size=2, q_length=6, kv_length=6, q_offset=0, kv_offset=0,
+              attention_mask=torch.tensor([[0, 0, 1, 1, 1, 1], [1] * 6]).bool(), device="cpu",
+              allow_is_causal_skip=False)
+    want = ALL_MASK_ATTENTION_FUNCTIONS["sdpa"](**kw)
+    assert torch.equal(made(**kw), want)
+    with G._QuantizedAttention(_Decoder(), _Cache(1.0)):
+        assert made(**kw) is None
+        other = []
+        _in_threads(lambda: other.append(made(**kw)))            # another thread's call
+        assert torch.equal(other[0], want)

@@ -49,7 +49,9 @@ class QuantizedKV(_Buffers):
     ``held`` (int32 [2, B, Hkv, 2]; K, V): which block each slot of the tails
     has, negative where that is not known.  ``allocate_quantized_kv`` makes it; a
     cache put together from buffers (``_replace`` among them) has none, and its
-    appends take the tails for the rows of whatever block they continue."""
+    appends take the tails for the rows of whatever block they continue.  Whoever
+    copies buffers into a cache that was in use copies ``held`` too, or fills it with
+    -1."""
 
     held: Optional[Tensor]
 
